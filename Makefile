@@ -13,7 +13,8 @@ LIBDIR     := fft_amd/lib
 BUILD      := build
 
 KERNEL_SRCS := $(CSRC)/inst_f32_a.hip $(CSRC)/inst_f32_b.hip $(CSRC)/inst_f32_c.hip \
-               $(CSRC)/inst_f16.hip $(CSRC)/inst_bf16.hip $(CSRC)/inst_tile.hip $(CSRC)/fourstep_twiddle.hip $(CSRC)/dist_kernels.hip $(CSRC)/fft_conv.hip $(CSRC)/tfft_c_api.hip
+               $(CSRC)/inst_f16.hip $(CSRC)/inst_bf16.hip $(CSRC)/inst_tile.hip $(CSRC)/fourstep_twiddle.hip $(CSRC)/dist_kernels.hip $(CSRC)/fft_conv.hip \
+               $(CSRC)/recurrence.hip $(CSRC)/rotary.hip $(CSRC)/tfft_c_api.hip
 KERNEL_OBJS := $(patsubst $(CSRC)/%.hip,$(BUILD)/%.o,$(KERNEL_SRCS))
 KERNEL_HDRS := $(wildcard $(CSRC)/*.hpp) include/thunderfft_c.h
 
@@ -39,6 +40,11 @@ $(BUILD)/%.o: $(CSRC)/%.hip $(KERNEL_HDRS)
 # straight-line kernel gains from it too (A/B of four builds of this unit: max-ilp 78.9 / 75.0 % at N = 8192 / 16384,
 # the default strategy 76.6 / 73.6, max-memory-clause 75.5 / 74.0, iterative-minreg 74.3 / 32.3).
 FLAGS_inst_f32_c := -mllvm -amdgpu-sched-strategy=max-ilp
+
+# The sequence operators are written in plain fp32 arithmetic on short arrays, which the compiler would otherwise pair
+# into packed fp32 instructions by itself.
+FLAGS_recurrence := -Xclang -target-feature -Xclang -packed-fp32-ops
+FLAGS_rotary     := -Xclang -target-feature -Xclang -packed-fp32-ops
 
 $(LIB): $(KERNEL_OBJS)
 	@mkdir -p $(LIBDIR)

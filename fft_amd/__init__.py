@@ -21,4 +21,4 @@ from .api import (  # noqa: F401
     fft,
     SUPPORTED_N,
 )
-from . import conv, synth  # noqa: F401
+from . import conv, recurrence, rotary, synth  # noqa: F401

@@ -235,8 +235,10 @@ int finish_launch(hipStream_t s) {
 
 }  // namespace
 
-// error reporting for the translation units that hold only kernels and their argument checks (dist_kernels.hip)
+// error reporting for the translation units that hold only kernels and their argument checks (dist_kernels.hip,
+// recurrence.hip, rotary.hip), and the end of a launch there
 extern "C" int tfft_internal_fail(int code, const char* message) { return fail(code, "%s", message); }
+extern "C" int tfft_internal_finish(void* stream) { return finish_launch(static_cast<hipStream_t>(stream)); }
 
 extern "C" int tfft_fourstep_twiddle_launch(void* d_data, long long rows, long long cols, long long row0,
                                             long long col0, long long n, int forward, void* stream);

@@ -294,6 +294,118 @@ int tfft_conv_tiles_exec(int dtype, int n, const void* d_in, const void* d_hf, v
  * valid until tfft_finalize(dtype). */
 int tfft_get_twiddle_table(int dtype, int n, const void** d_table);
 
+/* Gated linear recurrence over sequences, per batch entry b and channel c:
+ *     h[t] = a[t] h[t - 1] + x[t],   y[t] = h[t],   t = 0 ... length - 1,   h[-1] = initial (0 where it is NULL),
+ * the operator the long convolution above becomes when the decay depends on the input (with a constant decay a it is
+ * the causal convolution with the taps a^k). No counterpart in the reference, whose convolutions have fixed taps.
+ *
+ * Element types: x, y and their gradients have `dtype`; the gate has `gate_dtype`, TFFT_F32 or `dtype`. States
+ * (initial, last and their gradients) are contiguous fp32 [batch][channels]; all arithmetic is fp32 and every output is
+ * rounded once. gate_form TFFT_GATE_DECAY: a = gate; TFFT_GATE_LOG: a = exp(gate), a gate of minus infinity restarts
+ * the recurrence. `share` consecutive channels share one gate: the gate has channels / share entries a step (share
+ * divides channels). |a| <= 1 is what the operator is made for; larger decays are computed as long as the product of
+ * the decays over the sequence stays finite in fp32.
+ *
+ * Layout: element strides (batch, time, channel; for the gate: batch, time, gate). Any non-negative strides are taken;
+ * inputs may repeat (stride 0), outputs may not. Layouts with kernels of their own are channel stride 1 ([batch][time]
+ * [channel] activations) and, for share == 1, time stride 1 (the convolution's [batch][channel][time] signals). x and y (dy and
+ * dx) may be the same buffer with the same strides; every other overlap of an output with anything gives wrong results.
+ *
+ * lengths (NULL, or int32 [batch] on the device, clamped to 0 ... length): a padded batch. The steps behind a
+ * sequence's length leave its state as it is and are not read (NaN there does no harm); y, dx and dgate are 0 there.
+ * A sequence of length 0 has last = initial.
+ *
+ * Results do not depend on timing: the same call gives the same bits. Asynchronous on `stream`; allocates nothing.
+ * workspace: at least tfft_scan_workspace_bytes bytes of device memory, 8-byte aligned, that no other call uses until
+ * this one is done; its contents do not matter. */
+enum { TFFT_GATE_DECAY = 0, TFFT_GATE_LOG = 1 };
+typedef struct tfft_seq_view {
+  void* data; /* read only where the view is an input */
+  long long batch, time, channel;
+} tfft_seq_view;
+typedef struct tfft_scan_args {
+  int struct_size; /* sizeof(tfft_scan_args) */
+  int dtype, gate_dtype, gate_form;
+  long long batch, length, channels, share;
+  tfft_seq_view x, gate, y;
+  const int* lengths;   /* may be NULL */
+  const float* initial; /* may be NULL */
+  float* last;          /* h after the last step; may be NULL */
+  void* workspace;
+  unsigned long long workspace_bytes;
+} tfft_scan_args;
+int tfft_scan_forward(const tfft_scan_args* args, void* stream);
+
+/* Gradients of tfft_scan_forward from y as it was stored (rounded to dtype):
+ *     c[t] = a[t] (dy[t] + c[t + 1]),  c[length] = dlast (0 where it is NULL),
+ *     dx[t] = dy[t] + c[t + 1],  d a[t] = sum over the gate's channels of dx[t] y[t - 1],  y[-1] = initial,
+ *     dgate = d a (TFFT_GATE_DECAY) or a d a (TFFT_GATE_LOG),  dinitial = c[0].
+ * dgate has gate_dtype; its view has channels / share entries a step. */
+typedef struct tfft_scan_grad_args {
+  int struct_size; /* sizeof(tfft_scan_grad_args) */
+  int dtype, gate_dtype, gate_form;
+  long long batch, length, channels, share;
+  tfft_seq_view dy, y, gate, dx, dgate;
+  const int* lengths;   /* may be NULL */
+  const float* initial; /* may be NULL */
+  const float* dlast;   /* may be NULL */
+  float* dinitial;      /* may be NULL */
+  void* workspace;
+  unsigned long long workspace_bytes;
+} tfft_scan_grad_args;
+int tfft_scan_backward(const tfft_scan_grad_args* args, void* stream);
+
+/* Workspace of the two calls above for these arguments (data pointers are not looked at; sizes, types and strides are).
+ * Exactly one of forward and backward is given, the other is NULL. */
+int tfft_scan_workspace_bytes(const tfft_scan_args* forward, const tfft_scan_grad_args* backward,
+                              unsigned long long* bytes);
+
+/* One token of the recurrence for every sequence of a serving batch: new_state = a state + x, y = new_state rounded to
+ * dtype. Channel (gate) stride 1; the batch strides are given. state and new_state fp32, may be the same buffer (with
+ * the same stride); y may be x. */
+typedef struct tfft_scan_step_args {
+  int struct_size; /* sizeof(tfft_scan_step_args) */
+  int dtype, gate_dtype, gate_form;
+  long long batch, channels, share;
+  const void *x, *gate;
+  const float* state;
+  float* new_state;
+  void* y; /* may be NULL */
+  long long x_batch, gate_batch, state_batch, new_state_batch, y_batch;
+} tfft_scan_step_args;
+int tfft_scan_step(const tfft_scan_step_args* args, void* stream);
+
+/* Rotary positions: the pair (re, im) number i of every head of the token at position p becomes
+ *     magnitude * (re + i im) * exp(2 pi i p F[i]),    conjugated when inverse != 0 (which makes it the gradient),
+ * the product of tfft_fourstep_twiddle with frequencies and positions of the caller's. turns: rotary / 2 device words
+ * of 64 bits, the frequency in units of 2^-64 turns per position, round(2^64 f / 2 pi) for f radians per position: the
+ * product with a 64-bit position, taken modulo 2^64, is the phase to 2^-64 turns times the position, however far it is.
+ * pairs TFFT_PAIRS_HALF: values i and i + rotary / 2 of the head; TFFT_PAIRS_INTERLEAVED: values 2 i and 2 i + 1.
+ * Values behind the first `rotary` of a head are copied. Rotates one tensor or two (the second one's in NULL) by the
+ * same positions in one launch; element strides (batch, time, head), values of a head contiguous; out may be in with
+ * the same strides. positions: int64 or int32 (position_bytes 8 or 4) with strides, or NULL: first + t.
+ * Arithmetic fp32, rounded once. dtype as above. Asynchronous on `stream`; allocates nothing. */
+enum { TFFT_PAIRS_HALF = 0, TFFT_PAIRS_INTERLEAVED = 1 };
+typedef struct tfft_rotary_view {
+  const void* in;
+  void* out;
+  long long heads;
+  long long in_batch, in_time, in_head, out_batch, out_time, out_head;
+} tfft_rotary_view;
+typedef struct tfft_rotary_args {
+  int struct_size; /* sizeof(tfft_rotary_args) */
+  int dtype, pairs, inverse;
+  long long batch, length;
+  int head, rotary; /* values of a head, and how many of them are rotated (even) */
+  float magnitude;
+  int position_bytes;
+  const void* turns;
+  const void* positions; /* may be NULL */
+  long long position_batch, position_time, first;
+  tfft_rotary_view tensor[2];
+} tfft_rotary_args;
+int tfft_rotary(const tfft_rotary_args* args, void* stream);
+
 const char* tfft_last_error(void);
 
 #ifdef __cplusplus
