@@ -259,8 +259,9 @@ def run(state):
         if own:
             from fft_amd import rotary
 
-            return rotary.rotate(s["plan"], s["q"], s["k"], positions=s["positions"], pairs=s["pairs"],
-                                 inverse=s["inverse"])
+            turned = rotary.rotate(s["plan"], s["q"], s["k"], positions=s["positions"], pairs=s["pairs"],
+                                   inverse=s["inverse"])
+            return (turned, None) if s["k"] is None else turned
         angle = s["positions"][..., None].double() * s["frequencies"]
         if s["inverse"]:
             angle = -angle
