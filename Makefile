@@ -14,7 +14,7 @@ BUILD      := build
 
 KERNEL_SRCS := $(CSRC)/inst_f32_a.hip $(CSRC)/inst_f32_b.hip $(CSRC)/inst_f32_c.hip \
                $(CSRC)/inst_f16.hip $(CSRC)/inst_bf16.hip $(CSRC)/inst_tile.hip $(CSRC)/fourstep_twiddle.hip $(CSRC)/dist_kernels.hip $(CSRC)/fft_conv.hip \
-               $(CSRC)/recurrence.hip $(CSRC)/rotary.hip $(CSRC)/tfft_c_api.hip
+               $(CSRC)/recurrence.hip $(CSRC)/recurrence_rows.hip $(CSRC)/recurrence_signals.hip $(CSRC)/rotary.hip $(CSRC)/tfft_c_api.hip
 KERNEL_OBJS := $(patsubst $(CSRC)/%.hip,$(BUILD)/%.o,$(KERNEL_SRCS))
 KERNEL_HDRS := $(wildcard $(CSRC)/*.hpp) include/thunderfft_c.h
 
@@ -43,8 +43,11 @@ FLAGS_inst_f32_c := -mllvm -amdgpu-sched-strategy=max-ilp
 
 # The sequence operators are written in plain fp32 arithmetic on short arrays, which the compiler would otherwise pair
 # into packed fp32 instructions by itself.
-FLAGS_recurrence := -Xclang -target-feature -Xclang -packed-fp32-ops
-FLAGS_rotary     := -Xclang -target-feature -Xclang -packed-fp32-ops
+UNPACKED_FP32 := -Xclang -target-feature -Xclang -packed-fp32-ops
+FLAGS_recurrence         := $(UNPACKED_FP32)
+FLAGS_recurrence_rows    := $(UNPACKED_FP32)
+FLAGS_recurrence_signals := $(UNPACKED_FP32)
+FLAGS_rotary             := $(UNPACKED_FP32)
 
 $(LIB): $(KERNEL_OBJS)
 	@mkdir -p $(LIBDIR)

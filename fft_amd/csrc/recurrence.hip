@@ -1,75 +1,14 @@
 // Gated linear recurrence h[t] = a[t] h[t-1] + x[t] along the time axis: tfft_scan_forward, tfft_scan_backward and
 // tfft_scan_step. No counterpart in the reference.
-#include "seq_common.hpp"
+#include "recurrence_kernels.hpp"
 
 namespace {
 using namespace tfft_seq;
 
-template <class T, class G>
-__global__ __launch_bounds__(256) void scan_walk_fwd(tfft_scan_args p) {
-  const long long n = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (n >= p.batch * p.channels) return;
-  const long long b = n / p.channels, c = n % p.channels;
-  const T* x = (const T*)p.x.data + b * p.x.batch + c * p.x.channel;
-  const G* g = (const G*)p.gate.data + b * p.gate.batch + c / p.share * p.gate.channel;
-  T* y = (T*)p.y.data + b * p.y.batch + c * p.y.channel;
-  long long len = p.length;
-  if (p.lengths) len = p.lengths[b] < 0 ? 0 : p.lengths[b] < len ? p.lengths[b] : len;
-  float h = p.initial ? p.initial[n] : 0.0f;
-  for (long long t = 0; t < p.length; ++t) {
-    if (t < len) {
-      float a = to_f32(g[t * p.gate.time]);
-      if (p.gate_form == TFFT_GATE_LOG) a = expf(a);
-      h = fmaf(a, h, to_f32(x[t * p.x.time]));
-    }
-    y[t * p.y.time] = t < len ? from_f32<T>(h) : from_f32<T>(0.0f);
-  }
-  if (p.last) p.last[n] = h;
-}
-
-template <class T, class G>
-__global__ __launch_bounds__(256) void scan_walk_bwd(tfft_scan_grad_args p) {
-  const long long n = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (n >= p.batch * p.channels) return;
-  const long long b = n / p.channels, c = n % p.channels;
-  const T* dy = (const T*)p.dy.data + b * p.dy.batch + c * p.dy.channel;
-  const T* y = (const T*)p.y.data + b * p.y.batch + c * p.y.channel;
-  const G* g = (const G*)p.gate.data + b * p.gate.batch + c / p.share * p.gate.channel;
-  T* dx = (T*)p.dx.data + b * p.dx.batch + c * p.dx.channel;
-  long long len = p.length;
-  if (p.lengths) len = p.lengths[b] < 0 ? 0 : p.lengths[b] < len ? p.lengths[b] : len;
-  float carry = p.dlast ? p.dlast[n] : 0.0f;
-  for (long long t = p.length - 1; t >= 0; --t) {
-    float e = 0.0f, da = 0.0f;
-    if (t < len) {
-      float a = to_f32(g[t * p.gate.time]);
-      if (p.gate_form == TFFT_GATE_LOG) a = expf(a);
-      e = to_f32(dy[t * p.dy.time]) + carry;
-      const float before = t > 0 ? to_f32(y[(t - 1) * p.y.time]) : p.initial ? p.initial[n] : 0.0f;
-      da = e * before;
-      carry = a * e;
-      if (p.gate_form == TFFT_GATE_LOG) da *= a;
-    }
-    dx[t * p.dx.time] = from_f32<T>(e);
-    if (p.share == 1)
-      ((G*)p.dgate.data)[b * p.dgate.batch + t * p.dgate.time + c * p.dgate.channel] = from_f32<G>(da);
-    else
-      ((float*)p.workspace)[(b * p.length + t) * p.channels + c] = da;
-  }
-  if (p.dinitial) p.dinitial[n] = carry;
-}
-
-// dgate of a shared gate: its channels' terms, which lie side by side in the workspace, summed in their order
-template <class G>
-__global__ __launch_bounds__(256) void sum_shares(tfft_scan_grad_args p) {
-  const long long gates = p.channels / p.share;
-  const long long n = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (n >= p.batch * p.length * gates) return;
-  const long long g = n % gates, bt = n / gates, b = bt / p.length, t = bt % p.length;
-  const float* part = (const float*)p.workspace + bt * p.channels + g * p.share;
-  float sum = 0.0f;
-  for (long long i = 0; i < p.share; ++i) sum += part[i];
-  ((G*)p.dgate.data)[b * p.dgate.batch + t * p.dgate.time + g * p.dgate.channel] = from_f32<G>(sum);
+// The words that chunks hand their states on with, cleared by a kernel of the same call: it may be captured and
+// replayed, and nothing of an earlier call is left in them.
+__global__ __launch_bounds__(256) void clear_words(word* words, long long n) {
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) words[i] = 0;
 }
 
 template <class T, class G>
@@ -78,7 +17,7 @@ __global__ __launch_bounds__(256) void scan_step(tfft_scan_step_args p) {
   if (n >= p.batch * p.channels) return;
   const long long b = n / p.channels, c = n % p.channels;
   float a = to_f32(((const G*)p.gate)[b * p.gate_batch + c / p.share]);
-  if (p.gate_form == TFFT_GATE_LOG) a = expf(a);
+  if (p.gate_form == TFFT_GATE_LOG) a = exp_decay(a);
   const float h = fmaf(a, p.state[b * p.state_batch + c], to_f32(((const T*)p.x)[b * p.x_batch + c]));
   p.new_state[b * p.new_state_batch + c] = h;
   if (p.y) ((T*)p.y)[b * p.y_batch + c] = from_f32<T>(h);
@@ -86,13 +25,13 @@ __global__ __launch_bounds__(256) void scan_step(tfft_scan_step_args p) {
 
 // ---- argument checks ----------------------------------------------------------------------------------------------
 
-constexpr long long kMaxExtent = 0x7fffffffLL;
+constexpr long long kMaxExtent = 0x7fffffffLL, kMaxLength = 1LL << 30;
 
 const char* check_sizes(int dtype, int gate_dtype, int gate_form, long long batch, long long length, long long channels,
                         long long share) {
   if (gate_form != TFFT_GATE_DECAY && gate_form != TFFT_GATE_LOG) return "gate_form is TFFT_GATE_DECAY or TFFT_GATE_LOG";
   if (batch < 0 || length < 0 || channels < 0) return "negative extent";
-  if (batch > kMaxExtent || length > kMaxExtent || channels > kMaxExtent) return "an extent is 2^31 or more";
+  if (batch > kMaxExtent || length > kMaxLength || channels > kMaxExtent - 3) return "an extent is too large";
   if (share < 1 || channels % share) return "share does not divide the channels";
   return nullptr;
 }
@@ -152,22 +91,40 @@ const char* check_workspace(const void* p, unsigned long long bytes, unsigned lo
   return (reinterpret_cast<uintptr_t>(p) & 7u) ? "the workspace is not aligned to 8 bytes" : nullptr;
 }
 
-unsigned long long workspace_of(const tfft_scan_args& p) { return 0; }
-unsigned long long workspace_of(const tfft_scan_grad_args& p) {
-  return p.share > 1 ? 4ull * p.batch * p.length * p.channels : 0;
+// How a call runs. Steps side by side take the signals' kernels where channels do not lie side by side too; every other
+// layout goes through the rows' kernels, which take any strides.
+template <class P>
+bool as_signals(const P& p) {
+  return signals_fit(p) && !(rows_vector(p) && p.channels > 1);
+}
+template <class P>
+Chunking plan_of(const P& p) {
+  return as_signals(p) ? plan_signals(p) : plan_rows(p);
+}
+unsigned long long parts_of(const tfft_scan_args&) { return 0; }
+unsigned long long parts_of(const tfft_scan_grad_args& p) {
+  return !as_signals(p) && rows_sums_shares(p) ? 4ull * p.batch * p.length * p.channels : 0;
+}
+template <class P>
+unsigned long long workspace_of(const P& p) {
+  return 8ull * plan_of(p).words() + parts_of(p);
+}
+template <class P>
+const char* check_plan(const P& p) {
+  const char* large = "more sequences or steps than one launch takes";
+  if (p.batch * (p.channels + 3) > kMaxExtent || (p.share > 1 && (__int128)p.batch * p.length * p.channels > ((__int128)1 << 38)))
+    return large;
+  const Chunking c = plan_of(p);
+  return c.tiles * c.chunks > kMaxExtent ? large : nullptr;
+}
+
+template <class P>
+void clear(const Chunking& c, const P& p, hipStream_t s) {
+  const long long n = c.words();
+  if (n) clear_words<<<(unsigned)(n < 256 * 1024 ? (n + 255) / 256 : 1024), 256, 0, s>>>((word*)p.workspace, n);
 }
 
 unsigned blocks(long long threads) { return (unsigned)((threads + 255) / 256); }
-
-// f(T(), G()) for the element types of a call
-template <class F>
-void with_types(int dtype, int gate_dtype, F f) {
-  if (dtype == TFFT_F32) f(float(), float());
-  else if (dtype == TFFT_F16 && gate_dtype == TFFT_F32) f(f16(), float());
-  else if (dtype == TFFT_F16) f(f16(), f16());
-  else if (gate_dtype == TFFT_F32) f(bf16(), float());
-  else f(bf16(), bf16());
-}
 
 }  // namespace
 
@@ -180,10 +137,12 @@ extern "C" int tfft_scan_workspace_bytes(const tfft_scan_args* forward, const tf
   if (forward) {
     tfft_scan_args p = *forward;
     if (const int rc = check(who, &p)) return rc;
+    TFFT_SEQ_CHECK(check_plan(p));
     *bytes = workspace_of(p);
   } else {
     tfft_scan_grad_args p = *backward;
     if (const int rc = check(who, &p)) return rc;
+    TFFT_SEQ_CHECK(check_plan(p));
     *bytes = workspace_of(p);
   }
   return TFFT_OK;
@@ -194,6 +153,7 @@ extern "C" int tfft_scan_forward(const tfft_scan_args* args, void* stream) {
   if (!args || args->struct_size != (int)sizeof *args) return refuse(who, "null arguments, or struct_size is not theirs");
   tfft_scan_args p = *args;
   if (const int rc = check(who, &p)) return rc;
+  TFFT_SEQ_CHECK(check_plan(p));
   if (p.batch == 0 || p.channels == 0) return TFFT_OK;
   TFFT_SEQ_CHECK(check_view(p.x, p.dtype, p.batch, p.length, p.channels, false));
   TFFT_SEQ_CHECK(check_view(p.gate, p.gate_dtype, p.batch, p.length, p.channels / p.share, false));
@@ -201,9 +161,10 @@ extern "C" int tfft_scan_forward(const tfft_scan_args* args, void* stream) {
   for (const void* s : {(const void*)p.lengths, (const void*)p.initial, (const void*)p.last}) TFFT_SEQ_CHECK(check_state(s));
   TFFT_SEQ_CHECK(check_workspace(p.workspace, p.workspace_bytes, workspace_of(p)));
   hipStream_t s = static_cast<hipStream_t>(stream);
-  with_types(p.dtype, p.gate_dtype, [&](auto t, auto g) {
-    scan_walk_fwd<decltype(t), decltype(g)><<<blocks(p.batch * p.channels), 256, 0, s>>>(p);
-  });
+  const Chunking c = plan_of(p);
+  clear(c, p, s);
+  if (as_signals(p)) launch_signals(p, c, (word*)p.workspace, s);
+  else launch_rows(p, c, (word*)p.workspace, s);
   return tfft_internal_finish(stream);
 }
 
@@ -212,6 +173,7 @@ extern "C" int tfft_scan_backward(const tfft_scan_grad_args* args, void* stream)
   if (!args || args->struct_size != (int)sizeof *args) return refuse(who, "null arguments, or struct_size is not theirs");
   tfft_scan_grad_args p = *args;
   if (const int rc = check(who, &p)) return rc;
+  TFFT_SEQ_CHECK(check_plan(p));
   if (p.batch == 0 || p.channels == 0) return TFFT_OK;
   TFFT_SEQ_CHECK(check_view(p.dy, p.dtype, p.batch, p.length, p.channels, false));
   TFFT_SEQ_CHECK(check_view(p.y, p.dtype, p.batch, p.length, p.channels, false));
@@ -222,11 +184,10 @@ extern "C" int tfft_scan_backward(const tfft_scan_grad_args* args, void* stream)
     TFFT_SEQ_CHECK(check_state(s));
   TFFT_SEQ_CHECK(check_workspace(p.workspace, p.workspace_bytes, workspace_of(p)));
   hipStream_t s = static_cast<hipStream_t>(stream);
-  with_types(p.dtype, p.gate_dtype, [&](auto t, auto g) {
-    scan_walk_bwd<decltype(t), decltype(g)><<<blocks(p.batch * p.channels), 256, 0, s>>>(p);
-    if (p.share > 1 && p.length > 0)
-      sum_shares<decltype(g)><<<blocks(p.batch * p.length * (p.channels / p.share)), 256, 0, s>>>(p);
-  });
+  const Chunking c = plan_of(p);
+  clear(c, p, s);
+  if (as_signals(p)) launch_signals(p, c, (word*)p.workspace, s);
+  else launch_rows(p, c, (word*)p.workspace, (float*)((word*)p.workspace + c.words()), s);
   return tfft_internal_finish(stream);
 }
 

@@ -1,0 +1,260 @@
+// The gated linear recurrence where neighbouring steps lie side by side: the convolution's signals [batch][channel]
+// [time], one gate a channel.
+#include "recurrence_kernels.hpp"
+
+namespace tfft_seq {
+namespace {
+
+// A thread holds E consecutive steps of one row (batch entry, channel). Rows of up to 64 E steps: the next power of two
+// of lanes, several rows a wave. Longer rows: one a workgroup, in chunks of up to kMaxWaves waves.
+constexpr int kMaxWaves = 8, kMaxGroup = 64;
+constexpr int kSteps = 16;
+
+struct Shape {
+  long long rows;
+  int length, channels, log_gate;
+  int chunks, group, lanes;
+  word* words;
+};
+
+template <int E, class T>
+__device__ __forceinline__ Run<T, E> load_steps(const T* p, int t0, int len) {
+  return load_some<E>(p + t0, min(max(len - t0, 0), E));
+}
+template <int E, class T>
+__device__ __forceinline__ void store_steps(T* p, int t0, int length, const Run<T, E>& r) {
+  store_some<E>(p + t0, r, min(max(length - t0, 0), E));
+}
+
+// Decays of E steps; 1 behind the sequence. time is 1, or 0 for one decay throughout.
+template <int E, class G>
+__device__ __forceinline__ void load_decays(const G* g, long long time, int t0, int len, int log_gate, float (&a)[E]) {
+  if (time) {
+    const Run<G, E> r = load_steps<E>(g, t0, len);
+#pragma unroll
+    for (int i = 0; i < E; ++i) a[i] = r.get(i);
+  } else {
+    const float one = t0 < len ? to_f32(g[0]) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) a[i] = one;
+  }
+  if (log_gate) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) a[i] = exp_decay(a[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < E; ++i) a[i] = t0 + i < len ? a[i] : 1.0f;
+}
+
+// (A, B) of all pieces up to and with this thread's, among `width` threads that follow one another (a power of two,
+// or a whole wave), then those in front of it
+__device__ __forceinline__ void scan_lanes(int lane, int width, float& A, float& B, float& front_a, float& front_b) {
+  const int i = lane & (width - 1);
+  for (int d = 1; d < width; d *= 2) {
+    const float a = __shfl_up(A, d), b = __shfl_up(B, d);
+    if (i >= d) {
+      B = join(A, b, B);
+      A *= a;
+    }
+  }
+  front_a = __shfl_up(A, 1), front_b = __shfl_up(B, 1);
+  if (i == 0) front_a = 1.0f, front_b = 0.0f;
+}
+
+struct Lds {
+  float A[kMaxWaves], B[kMaxWaves], h;
+  unsigned ticket;
+};
+
+// The state in front of this thread's piece from its (A, B) and `h`, the state before the first chunk. `order`: 0 for the
+// thread that comes first.
+__device__ __forceinline__ float state_in_front(const Shape& f, Lds& lds, unsigned chunk, long long row, int order, float A, float B, float h) {
+  const int lane = order & 63, wave = order >> 6, waves = blockDim.x >> 6;
+  float front_a, front_b;
+  scan_lanes(lane, f.lanes, A, B, front_a, front_b);
+  if (f.lanes < 64 || (waves == 1 && f.chunks <= 1)) return join(front_a, h, front_b);
+  if (lane == 63) lds.A[wave] = A, lds.B[wave] = B;
+  __syncthreads();
+  float wave_a = 1.0f, wave_b = 0.0f;
+  for (int w = 0; w < wave; ++w) {
+    wave_b = join(lds.A[w], wave_b, lds.B[w]);
+    wave_a *= lds.A[w];
+  }
+  if (f.chunks > 1) {
+    if (wave == waves - 1) {
+      const int r = chunk % f.group, q = chunk / f.group;
+      const bool more = chunk + 1 < (unsigned)f.chunks;
+      word* own = f.words + 1 + 2 * (row * f.chunks + chunk);
+      word* states = f.words + 1 + 2 * f.rows * f.chunks + row * ((f.chunks + f.group - 1) / f.group);
+      const float chunk_a = wave_a * lds.A[wave], chunk_b = join(lds.A[wave], wave_b, lds.B[wave]);
+      if (more && r != f.group - 1 && lane == 0) publish(own, chunk_a), publish(own + 1, chunk_b);
+      // lane k joins the k-th chunk of the group, those of this one's past are read together
+      float a = 1.0f, b = 0.0f, fa, fb;
+      if (lane < r) a = await(own - 2 * (r - lane)), b = await(own - 2 * (r - lane) + 1);
+      scan_lanes(lane, 64, a, b, fa, fb);
+      a = __shfl(a, 63), b = __shfl(b, 63);
+      if (q > 0) h = await(states + q - 1);
+      h = join(a, h, b);
+      if (more && r == f.group - 1 && lane == 0) publish(states + q, join(chunk_a, h, chunk_b));
+      if (lane == 0) lds.h = h;
+    }
+    __syncthreads();
+    h = lds.h;
+  }
+  h = join(wave_a, h, wave_b);
+  return join(front_a, h, front_b);
+}
+
+// Row and chunk of this thread; a ticket where chunks depend on each other
+__device__ __forceinline__ void take(const Shape& f, Lds& lds, long long* row, unsigned* chunk) {
+  if (f.chunks <= 1) {
+    *chunk = 0;
+    *row = f.lanes < 64 ? ((long long)blockIdx.x * blockDim.x + threadIdx.x) / f.lanes : (long long)blockIdx.x;
+    return;
+  }
+  if (threadIdx.x == 0) lds.ticket = (unsigned)__hip_atomic_fetch_add(f.words, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  *chunk = lds.ticket / (unsigned)f.rows;
+  *row = lds.ticket % (unsigned)f.rows;
+}
+
+template <class T, class G>
+__global__ __launch_bounds__(64 * kMaxWaves) void scan_signals_fwd(tfft_scan_args p, Shape f) {
+  constexpr int E = kSteps;
+  __shared__ Lds lds;
+  long long row;
+  unsigned chunk;
+  take(f, lds, &row, &chunk);
+  const bool live = row < f.rows;
+  if (!live) row = 0;
+  const int b = (int)(row / f.channels), c = (int)(row % f.channels);
+  const int order = threadIdx.x, piece = f.lanes < 64 ? order & (f.lanes - 1) : order;
+  const int t0 = (int)(chunk * blockDim.x + piece) * E, len = live ? steps_of(p.lengths, b, f.length) : 0;
+  const T* x = (const T*)p.x.data + b * p.x.batch + c * p.x.channel;
+  const G* g = (const G*)p.gate.data + b * p.gate.batch + c * p.gate.channel;
+  const Run<T, E> xr = load_steps<E>(x, t0, len);
+  float a[E];
+  load_decays<E>(g, p.gate.time, t0, len, f.log_gate, a);
+  float h = p.initial ? p.initial[row] : 0.0f;
+  float A = 1.0f, B = 0.0f;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    A *= a[i];
+    B = fmaf(a[i], B, xr.get(i));
+  }
+  h = state_in_front(f, lds, chunk, row, order, A, B, h);
+  Run<T, E> r;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    h = fmaf(a[i], h, xr.get(i));
+    r.set(i, t0 + i < len ? h : 0.0f);
+  }
+  if (live) store_steps<E>((T*)p.y.data + b * p.y.batch + c * p.y.channel, t0, f.length, r);
+  const int pieces = f.lanes < 64 ? f.lanes : (int)blockDim.x;
+  if (p.last && live && chunk + 1 == (unsigned)f.chunks && piece == pieces - 1) p.last[row] = h;
+}
+
+// Backwards in time: the first thread has the latest steps, chunk 0 is the latest
+template <class T, class G>
+__global__ __launch_bounds__(64 * kMaxWaves) void scan_signals_bwd(tfft_scan_grad_args p, Shape f) {
+  constexpr int E = kSteps;
+  __shared__ Lds lds;
+  long long row;
+  unsigned chunk;
+  take(f, lds, &row, &chunk);
+  const bool live = row < f.rows;
+  if (!live) row = 0;
+  const int b = (int)(row / f.channels), c = (int)(row % f.channels);
+  const int order = threadIdx.x, piece = f.lanes < 64 ? order & (f.lanes - 1) : order;
+  const int pieces = f.lanes < 64 ? f.lanes : (int)blockDim.x;
+  const int t0 = ((int)(f.chunks - 1 - chunk) * pieces + pieces - 1 - piece) * E, len = live ? steps_of(p.lengths, b, f.length) : 0;
+  const T* dy = (const T*)p.dy.data + b * p.dy.batch + c * p.dy.channel;
+  const T* y = (const T*)p.y.data + b * p.y.batch + c * p.y.channel;
+  const G* g = (const G*)p.gate.data + b * p.gate.batch + c * p.gate.channel;
+  const Run<T, E> d = load_steps<E>(dy, t0, len), own = load_steps<E>(y, t0, len);
+  const T before = t0 > 0 && t0 - 1 < len ? y[t0 - 1] : from_f32<T>(0.0f);
+  float a[E];
+  load_decays<E>(g, p.gate.time, t0, len, f.log_gate, a);
+  const float start = p.initial ? p.initial[row] : 0.0f;
+  float A = 1.0f, B = 0.0f;
+#pragma unroll
+  for (int i = E - 1; i >= 0; --i) {
+    A *= a[i];
+    B = a[i] * (B + d.get(i));
+  }
+  float k = state_in_front(f, lds, chunk, row, order, A, B, p.dlast ? p.dlast[row] : 0.0f);
+  float dx[E], dgate[E];
+#pragma unroll
+  for (int i = E - 1; i >= 0; --i) {
+    const float e = d.get(i) + k;
+    const float state = i > 0 ? own.get(i > 0 ? i - 1 : 0) : t0 > 0 ? to_f32(before) : start;
+    const bool inside = t0 + i < len;
+    dgate[i] = inside ? e * state * (f.log_gate ? a[i] : 1.0f) : 0.0f;
+    dx[i] = inside ? e : 0.0f;
+    k = a[i] * e;
+  }
+  Run<T, E> r;
+  Run<G, E> q;
+#pragma unroll
+  for (int i = 0; i < E; ++i) r.set(i, dx[i]), q.set(i, dgate[i]);
+  if (live) {
+    store_steps<E>((T*)p.dx.data + b * p.dx.batch + c * p.dx.channel, t0, f.length, r);
+    store_steps<E>((G*)p.dgate.data + b * p.dgate.batch + c * p.dgate.channel, t0, f.length, q);
+  }
+  if (p.dinitial && live && chunk + 1 == (unsigned)f.chunks && piece == pieces - 1) p.dinitial[row] = k;
+}
+
+Chunking plan(long long batch, long long length, long long channels) {
+  Chunking c;
+  const long long rows = batch * channels, pieces = (length + kSteps - 1) / kSteps;
+  c.tiles = rows;
+  c.state_words = rows;
+  c.group = kMaxGroup;
+  if (pieces <= 32) {
+    c.lanes = 1;
+    while (c.lanes < pieces) c.lanes *= 2;
+    c.waves = 4;
+    c.chunks = 1;
+    return c;
+  }
+  c.waves = (int)(pieces > 64 * (kMaxWaves - 1) ? kMaxWaves : (pieces + 63) / 64);
+  c.chunks = (pieces + 64 * c.waves - 1) / (64 * c.waves);
+  return c;
+}
+
+template <class P>
+Shape shape_of(const P& p, const Chunking& c, word* words) {
+  return Shape{p.batch * p.channels, (int)p.length, (int)p.channels, p.gate_form == TFFT_GATE_LOG,
+               (int)c.chunks, c.group, c.lanes, words};
+}
+
+dim3 grid_of(const Chunking& c) {
+  const long long per_block = c.lanes < 64 ? 64 * c.waves / c.lanes : 1;
+  return dim3((unsigned)((c.tiles + per_block - 1) / per_block * c.chunks));
+}
+
+}  // namespace
+
+bool signals_fit(const tfft_scan_args& p) {
+  return p.share == 1 && p.x.time == 1 && p.y.time == 1 && p.gate.time <= 1;
+}
+bool signals_fit(const tfft_scan_grad_args& p) {
+  return p.share == 1 && p.dy.time == 1 && p.y.time == 1 && p.dx.time == 1 && p.dgate.time == 1 && p.gate.time <= 1;
+}
+Chunking plan_signals(const tfft_scan_args& p) { return plan(p.batch, p.length, p.channels); }
+Chunking plan_signals(const tfft_scan_grad_args& p) { return plan(p.batch, p.length, p.channels); }
+
+void launch_signals(const tfft_scan_args& p, const Chunking& c, word* words, hipStream_t s) {
+  const Shape f = shape_of(p, c, words);
+  with_types(p.dtype, p.gate_dtype, [&](auto t, auto g) {
+    scan_signals_fwd<decltype(t), decltype(g)><<<grid_of(c), dim3(64 * c.waves), 0, s>>>(p, f);
+  });
+}
+void launch_signals(const tfft_scan_grad_args& p, const Chunking& c, word* words, hipStream_t s) {
+  const Shape f = shape_of(p, c, words);
+  with_types(p.dtype, p.gate_dtype, [&](auto t, auto g) {
+    scan_signals_bwd<decltype(t), decltype(g)><<<grid_of(c), dim3(64 * c.waves), 0, s>>>(p, f);
+  });
+}
+
+}  // namespace tfft_seq

@@ -24,21 +24,83 @@ __device__ __forceinline__ T from_f32(float v) {
   return (T)v;  // round to nearest even, the one rounding of an output
 }
 
-// N consecutive elements. The copies go through memcpy: the elements' addresses are multiples of the element size
-// only (a row of 770 halves, a slice at an odd offset), and gfx950 loads and stores dwords at any address.
+// exp of a log decay: one product and the chip's 2^x. Off by one unit in the last place of 2^x and by |x| 1.3 half units
+// of the rounded product and factor, which a decay worth keeping (|x| below 20) does not notice; it takes 5 issue slots where expf takes
+// more than 20, and the scan's vector units are as busy as its memory.
+__device__ __forceinline__ float exp_decay(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
+
+// N consecutive elements, 16-bit ones two to a register. The copies go through memcpy: the elements' addresses are multiples
+// of the element size only (a row of 770 halves, a slice at an odd offset), and gfx950 loads and stores dwords at any
+// address.
 template <class T, int N>
 struct Run {
-  T v[N];
+  static constexpr bool kHalf = sizeof(T) == 2;
+  uint32_t w[kHalf ? (N + 1) / 2 : N];
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (!kHalf) {
+      return __uint_as_float(w[i]);
+    } else {
+      const uint16_t bits = (uint16_t)(w[i / 2] >> (i % 2 * 16));
+      T v;
+      __builtin_memcpy(&v, &bits, 2);
+      return (float)v;
+    }
+  }
+  // element i of an array filled in ascending order, rounded to nearest even: the one rounding of an output
+  __device__ __forceinline__ void set(int i, float f) {
+    const T v = (T)f;
+    if constexpr (!kHalf) {
+      w[i] = __float_as_uint(v);
+    } else {
+      uint16_t bits;
+      __builtin_memcpy(&bits, &v, 2);
+      if (i % 2 == 0) w[i / 2] = bits;
+      else w[i / 2] |= (uint32_t)bits << 16;
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (uint32_t& word : w) word = 0;
+  }
 };
 template <class T, int N>
 __device__ __forceinline__ Run<T, N> load_run(const T* p) {
   Run<T, N> r;
-  __builtin_memcpy(&r, p, sizeof(r));
+  if constexpr (sizeof(r) != N * sizeof(T)) r.clear();
+  __builtin_memcpy(r.w, p, N * sizeof(T));
   return r;
 }
 template <class T, int N>
 __device__ __forceinline__ void store_run(T* p, const Run<T, N>& r) {
-  __builtin_memcpy(p, &r, sizeof(r));
+  __builtin_memcpy(p, r.w, N * sizeof(T));
+}
+
+// The first `valid` of N elements, zeros behind them
+template <int N, class T>
+__device__ __forceinline__ Run<T, N> load_some(const T* p, int valid) {
+  if (valid == N) return load_run<T, N>(p);
+  Run<T, N> r;
+  r.clear();
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < valid) {
+      const Run<T, 1> one = load_run<T, 1>(p + i);
+      if constexpr (sizeof(T) == 4) r.w[i] = one.w[0];
+      else r.w[i / 2] |= one.w[0] << (i % 2 * 16);
+    }
+  return r;
+}
+template <int N, class T>
+__device__ __forceinline__ void store_some(T* p, const Run<T, N>& r, int valid) {
+  if (valid == N) return store_run<T, N>(p, r);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < valid) {
+      Run<T, 1> one;
+      if constexpr (sizeof(T) == 4) one.w[0] = r.w[i];
+      else one.w[0] = r.w[i / 2] >> (i % 2 * 16);
+      store_run<T, 1>(p + i, one);
+    }
 }
 
 inline bool misaligned(const void* p, int dtype) {
