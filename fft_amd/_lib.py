@@ -1,6 +1,7 @@
 """ctypes binding of libthunderfft_hip.so (C ABI declared in include/thunderfft_c.h)."""
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # THUNDERFFT_HIP_LIB: another build of the same library (A/B timing of two builds, an installed copy); it must export
@@ -83,49 +84,14 @@ class DistRadixArgs(ctypes.Structure):
         (k, ctypes.c_longlong) for k in ("rows", "row_len", "in_chunk", "in_pitch", "out_chunk", "out_pitch")]
 
 
-class SeqView(ctypes.Structure):
-    """tfft_seq_view of include/thunderfft_c.h."""
-    _fields_ = [("data", ctypes.c_void_p)] + [(k, ctypes.c_longlong) for k in ("batch", "time", "channel")]
-
-
-_SCAN_HEAD = [(k, ctypes.c_int) for k in ("struct_size", "dtype", "gate_dtype", "gate_form")] + [
-    (k, ctypes.c_longlong) for k in ("batch", "length", "channels", "share")]
-_SCAN_TAIL = [("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_ulonglong)]
-
-
-class ScanArgs(ctypes.Structure):
-    """tfft_scan_args of include/thunderfft_c.h."""
-    _fields_ = _SCAN_HEAD + [(k, SeqView) for k in ("x", "gate", "y")] + [
-        (k, ctypes.c_void_p) for k in ("lengths", "initial", "last")] + _SCAN_TAIL
-
-
-class ScanGradArgs(ctypes.Structure):
-    """tfft_scan_grad_args of include/thunderfft_c.h."""
-    _fields_ = _SCAN_HEAD + [(k, SeqView) for k in ("dy", "y", "gate", "dx", "dgate")] + [
-        (k, ctypes.c_void_p) for k in ("lengths", "initial", "dlast", "dinitial")] + _SCAN_TAIL
-
-
-class ScanStepArgs(ctypes.Structure):
-    """tfft_scan_step_args of include/thunderfft_c.h."""
-    _fields_ = [(k, ctypes.c_int) for k in ("struct_size", "dtype", "gate_dtype", "gate_form")] + [
-        (k, ctypes.c_longlong) for k in ("batch", "channels", "share")] + [
-        (k, ctypes.c_void_p) for k in ("x", "gate", "state", "new_state", "y")] + [
-        (k, ctypes.c_longlong) for k in ("x_batch", "gate_batch", "state_batch", "new_state_batch", "y_batch")]
-
-
-class RotaryView(ctypes.Structure):
-    """tfft_rotary_view of include/thunderfft_c.h."""
-    _fields_ = [("in_", ctypes.c_void_p), ("out", ctypes.c_void_p)] + [
-        (k, ctypes.c_longlong) for k in ("heads", "in_batch", "in_time", "in_head", "out_batch", "out_time", "out_head")]
-
-
-class RotaryArgs(ctypes.Structure):
-    """tfft_rotary_args of include/thunderfft_c.h."""
-    _fields_ = [(k, ctypes.c_int) for k in ("struct_size", "dtype", "pairs", "inverse")] + [
-        ("batch", ctypes.c_longlong), ("length", ctypes.c_longlong), ("head", ctypes.c_int), ("rotary", ctypes.c_int),
-        ("magnitude", ctypes.c_float), ("position_bytes", ctypes.c_int), ("turns", ctypes.c_void_p),
-        ("positions", ctypes.c_void_p)] + [
-        (k, ctypes.c_longlong) for k in ("position_batch", "position_time", "first")] + [("tensor", RotaryView * 2)]
+# The argument structures of the sequence operators, packed into bytes: a tenth of the time that filling a
+# ctypes.Structure takes, in calls of which a decoder makes one for every layer and token. A view is its pointer and its strides
+# (batch, time, channel).
+_SCAN = "@4i4q%s%s"
+SCAN_ARGS = struct.Struct(_SCAN % ("P3q" * 3, "3PPQ"))           # tfft_scan_args
+SCAN_GRAD_ARGS = struct.Struct(_SCAN % ("P3q" * 5, "4PPQ"))      # tfft_scan_grad_args
+SCAN_STEP_ARGS = struct.Struct("@4i3q5P5q")                      # tfft_scan_step_args
+ROTARY_ARGS = struct.Struct("@4i2q2ifi2P3q" + "2P7q" * 2)        # tfft_rotary_args
 
 
 _lib = None
@@ -172,11 +138,11 @@ def load():
     lib.tfft_conv_forget_layout.argtypes = [vp, ctypes.c_ulonglong]
     lib.tfft_conv_tiles_exec.argtypes = [i, i, vp, vp, vp, ll, ll, i, vp]
     lib.tfft_get_twiddle_table.argtypes = [i, i, ctypes.POINTER(vp)]
-    lib.tfft_scan_forward.argtypes = [ctypes.POINTER(ScanArgs), vp]
-    lib.tfft_scan_backward.argtypes = [ctypes.POINTER(ScanGradArgs), vp]
-    lib.tfft_scan_workspace_bytes.argtypes = [ctypes.POINTER(ScanArgs), ctypes.POINTER(ScanGradArgs), ullp]
-    lib.tfft_scan_step.argtypes = [ctypes.POINTER(ScanStepArgs), vp]
-    lib.tfft_rotary.argtypes = [ctypes.POINTER(RotaryArgs), vp]
+    lib.tfft_scan_forward.argtypes = [cp, vp]
+    lib.tfft_scan_backward.argtypes = [cp, vp]
+    lib.tfft_scan_workspace_bytes.argtypes = [cp, cp, ullp]
+    lib.tfft_scan_step.argtypes = [cp, vp]
+    lib.tfft_rotary.argtypes = [cp, vp]
     lib.tfft_last_error.argtypes = []
     lib.tfft_last_error.restype = cp
     for name in SYMBOLS:

@@ -24,9 +24,16 @@ def _refuse(message, code=3):
     raise ThunderFFTError(code, message)
 
 
-def _on_stream(device, stream):
-    """What a call allocates belongs to the stream that it runs on."""
-    return torch.cuda.stream(torch.cuda.current_stream(device) if stream is None else stream)
+def _placed(call, device, stream, *args):
+    """call(*args, raw stream) with torch's current device and stream those of the call, so that what it allocates belongs to
+    the stream that it runs on. Switching costs more than a short kernel, so it is left out where nothing changes."""
+    if stream is None and device.index == torch.cuda.current_device():
+        return call(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    with torch.cuda.device(device):
+        if stream is None:
+            return call(*args, torch.cuda.current_stream(device).cuda_stream)
+        with torch.cuda.stream(stream):
+            return call(*args, stream.cuda_stream)
 
 
 def _types(who, x, gate):
@@ -41,30 +48,32 @@ def _types(who, x, gate):
 def _same_device(who, x, *others):
     if not x.is_cuda:
         _refuse(f"{who} needs device tensors")
+    device = x.device
     for t in others:
-        if t is not None and t.device != x.device:
-            _refuse(f"{who}: tensors on {x.device} and {t.device}")
+        if t is not None and t.device != device:
+            _refuse(f"{who}: tensors on {device} and {t.device}")
+    return device
 
 
 def _state(who, name, t, B, D):
     if t is None:
-        return None
-    if t.dtype != torch.float32 or tuple(t.shape) != (B, D) or not t.is_contiguous():
+        return 0
+    if t.dtype != torch.float32 or t.shape != (B, D) or not t.is_contiguous():
         _refuse(f"{who}: {name} is a contiguous float32 tensor [{B}, {D}]")
     return t.data_ptr()
 
 
 def _lengths(who, t, B):
     if t is None:
-        return None
-    if t.dtype != torch.int32 or tuple(t.shape) != (B,) or not t.is_contiguous():
+        return 0
+    if t.dtype != torch.int32 or t.shape != (B,) or not t.is_contiguous():
         _refuse(f"{who}: lengths is a contiguous int32 tensor [{B}]")
     return t.data_ptr()
 
 
 def _view(t, dim):
     b, p, q = t.stride()
-    return _lib.SeqView(t.data_ptr(), b, p, q) if dim == 1 else _lib.SeqView(t.data_ptr(), b, q, p)
+    return (t.data_ptr(), b, p, q) if dim == 1 else (t.data_ptr(), b, q, p)
 
 
 def _sizes(who, x, gate, dim):
@@ -72,34 +81,37 @@ def _sizes(who, x, gate, dim):
         _refuse(f"{who}: dim is 1 ([batch, time, channel]) or 2 ([batch, channel, time]), not {dim}")
     if x.dim() != 3 or gate.dim() != 3:
         _refuse(f"{who} needs tensors of three dimensions, got {tuple(x.shape)} and {tuple(gate.shape)}")
-    B, L, D = x.shape[0], x.shape[dim], x.shape[3 - dim]
-    G = gate.shape[3 - dim]
-    if gate.shape[0] != B or gate.shape[dim] != L or G < 1 and D > 0 or G > 0 and D % G:
-        _refuse(f"{who}: gate {tuple(gate.shape)} does not fit {tuple(x.shape)}: the same batch and time, and a number "
-                "of gates that divides the channels")
+    shape, gates = x.shape, gate.shape
+    B, L, D, G = shape[0], shape[dim], shape[3 - dim], gates[3 - dim]
+    if gates[0] != B or gates[dim] != L or (D > 0 if G < 1 else D % G):
+        _refuse(f"{who}: gate {tuple(gates)} does not fit {tuple(shape)}: the same batch and time, and a number of gates "
+                "that divides the channels")
     return B, L, D, (D // G if G else 1)
 
 
-def _out(who, name, t, like, dtype):
+def _out(who, name, t, like):
     if t is None:
-        return torch.empty(like, dtype=dtype[0], device=dtype[1])
-    if t.dtype != dtype[0] or tuple(t.shape) != tuple(like) or t.device != dtype[1]:
-        _refuse(f"{who}: {name} is a {dtype[0]} tensor {tuple(like)} on {dtype[1]}")
+        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    if t.dtype != like.dtype or t.shape != like.shape:
+        _refuse(f"{who}: {name} is a {like.dtype} tensor {tuple(like.shape)}")
     return t
 
 
-def _run(function, args, device, stream):
+def _run(function, packer, values, forward, device, stream):
     """Workspace and launch; torch's current device and stream are already those of the call."""
     lib = _lib.load()
-    need = ctypes.c_ulonglong(0)
-    forward = args if isinstance(args, _lib.ScanArgs) else None
-    backward = None if forward is not None else args
-    _check(lib.tfft_scan_workspace_bytes(forward, backward, need))
+    need = ctypes.c_ulonglong()
+    args = packer.pack(*values, 0, 0)
+    rc = lib.tfft_scan_workspace_bytes(args if forward else None, None if forward else args, need)
+    if rc:
+        _check(rc)
     if need.value:
         # from torch's allocator on the call's stream: it is reused in stream order, and within a graph's own pool
         workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
-        args.workspace, args.workspace_bytes = workspace.data_ptr(), need.value
-    _check(function(args, stream))
+        args = packer.pack(*values, workspace.data_ptr(), need.value)
+    rc = function(args, stream)
+    if rc:
+        _check(rc)
 
 
 def gated_scan(x, gate, dim=1, log_gate=False, lengths=None, initial=None, out=None, stream=None):
@@ -109,17 +121,19 @@ def gated_scan(x, gate, dim=1, log_gate=False, lengths=None, initial=None, out=N
     channels, one for D / G neighbours, of x's type or float32; with log_gate the decay is exp(gate). lengths (int32
     [B]): steps behind a sequence's length are not read, leave the state as it is, and y is 0 there. initial: fp32
     [B, D]. out: a tensor for y, x itself allowed. Asynchronous on `stream` (default: torch's current stream)."""
+    return _placed(_gated_scan, _same_device("gated_scan", x, gate, lengths, initial, out), stream, x, gate, dim, log_gate,
+                   lengths, initial, out)
+
+
+def _gated_scan(x, gate, dim, log_gate, lengths, initial, out, stream):
     who = "gated_scan"
-    _same_device(who, x, gate, lengths, initial, out)
     code, gate_code = _types(who, x, gate)
     B, L, D, share = _sizes(who, x, gate, dim)
-    with torch.cuda.device(x.device), _on_stream(x.device, stream):
-        y = _out(who, "out", out, x.shape, (x.dtype, x.device))
-        last = torch.empty(B, D, dtype=torch.float32, device=x.device)
-        args = _lib.ScanArgs(ctypes.sizeof(_lib.ScanArgs), code, gate_code, int(bool(log_gate)), B, L, D, share,
-                             _view(x, dim), _view(gate, dim), _view(y, dim), _lengths(who, lengths, B),
-                             _state(who, "initial", initial, B, D), last.data_ptr())
-        _run(_lib.load().tfft_scan_forward, args, x.device, torch.cuda.current_stream().cuda_stream)
+    y = _out(who, "out", out, x)
+    last = torch.empty((B, D), dtype=torch.float32, device=x.device)
+    _run(_lib.load().tfft_scan_forward, _lib.SCAN_ARGS,
+         (_lib.SCAN_ARGS.size, code, gate_code, bool(log_gate), B, L, D, share, *_view(x, dim), *_view(gate, dim), *_view(y, dim),
+          _lengths(who, lengths, B), _state(who, "initial", initial, B, D), last.data_ptr()), True, x.device, stream)
     return y, last
 
 
@@ -131,21 +145,23 @@ def gated_scan_backward(dy, y, gate, dim=1, log_gate=False, lengths=None, initia
     gate, dim, log_gate, lengths, initial: as the forward call had them. dgate has the gate's shape and type (the
     gradient of a gate that was broadcast by strides of 0 is the sum of it over those dimensions); dx and dgate may be
     given, dx may be dy. dinitial: fp32 [B, D]."""
+    return _placed(_gated_scan_backward,
+                   _same_device("gated_scan_backward", dy, y, gate, lengths, initial, dlast, dx, dgate), stream,
+                   dy, y, gate, dim, log_gate, lengths, initial, dlast, dx, dgate)
+
+
+def _gated_scan_backward(dy, y, gate, dim, log_gate, lengths, initial, dlast, dx, dgate, stream):
     who = "gated_scan_backward"
-    _same_device(who, dy, y, gate, lengths, initial, dlast, dx, dgate)
     code, gate_code = _types(who, dy, gate)
     B, L, D, share = _sizes(who, dy, gate, dim)
     if y.dtype != dy.dtype or y.shape != dy.shape:
         _refuse(f"{who}: y is a {dy.dtype} tensor {tuple(dy.shape)} like dy")
-    with torch.cuda.device(dy.device), _on_stream(dy.device, stream):
-        dx = _out(who, "dx", dx, dy.shape, (dy.dtype, dy.device))
-        dgate = _out(who, "dgate", dgate, gate.shape, (gate.dtype, gate.device))
-        dinitial = torch.empty(B, D, dtype=torch.float32, device=dy.device)
-        args = _lib.ScanGradArgs(ctypes.sizeof(_lib.ScanGradArgs), code, gate_code, int(bool(log_gate)), B, L, D, share,
-                                 _view(dy, dim), _view(y, dim), _view(gate, dim), _view(dx, dim), _view(dgate, dim),
-                                 _lengths(who, lengths, B), _state(who, "initial", initial, B, D),
-                                 _state(who, "dlast", dlast, B, D), dinitial.data_ptr())
-        _run(_lib.load().tfft_scan_backward, args, dy.device, torch.cuda.current_stream().cuda_stream)
+    dx, dgate = _out(who, "dx", dx, dy), _out(who, "dgate", dgate, gate)
+    dinitial = torch.empty((B, D), dtype=torch.float32, device=dy.device)
+    _run(_lib.load().tfft_scan_backward, _lib.SCAN_GRAD_ARGS,
+         (_lib.SCAN_GRAD_ARGS.size, code, gate_code, bool(log_gate), B, L, D, share, *_view(dy, dim), *_view(y, dim),
+          *_view(gate, dim), *_view(dx, dim), *_view(dgate, dim), _lengths(who, lengths, B), _state(who, "initial", initial, B, D),
+          _state(who, "dlast", dlast, B, D), dinitial.data_ptr()), False, dy.device, stream)
     return dx, dgate, dinitial
 
 
@@ -153,28 +169,34 @@ def gated_scan_step(x, gate, state, log_gate=False, new_state=None, out=None, st
     """y [B, D]: one token of the recurrence for every sequence. x: [B, D]; gate: [B, G]; state: fp32 [B, D], updated
     in place, or left as it is where new_state (fp32 [B, D]) is given. Rows may lie apart (any batch stride), the
     values of a row are contiguous."""
+    return _placed(_gated_scan_step, _same_device("gated_scan_step", x, gate, state, new_state, out), stream, x, gate, state,
+                   log_gate, new_state, out)
+
+
+def _gated_scan_step(x, gate, state, log_gate, new_state, out, stream):
     who = "gated_scan_step"
-    _same_device(who, x, gate, state, new_state, out)
     code, gate_code = _types(who, x, gate)
     if x.dim() != 2 or gate.dim() != 2 or gate.shape[0] != x.shape[0]:
         _refuse(f"{who} needs x [B, D] and gate [B, G], got {tuple(x.shape)} and {tuple(gate.shape)}")
     B, D = x.shape
     G = gate.shape[1]
-    if G < 1 and D > 0 or G > 0 and D % G:
+    if D > 0 if G < 1 else D % G:
         _refuse(f"{who}: {G} gates do not divide {D} channels")
     if new_state is None:
         new_state = state
-    for name, t in (("state", state), ("new_state", new_state)):
+    for t in (state, new_state):
         if t.dtype != torch.float32 or t.shape != x.shape:
-            _refuse(f"{who}: {name} is a float32 tensor [{B}, {D}]")
-    with torch.cuda.device(x.device), _on_stream(x.device, stream):
-        y = _out(who, "out", out, x.shape, (x.dtype, x.device))
-        for t in (x, gate, state, new_state, y):
-            if t.shape[1] > 1 and t.stride(1) != 1:
-                _refuse(f"{who}: the values of a row are contiguous")
-        args = _lib.ScanStepArgs(ctypes.sizeof(_lib.ScanStepArgs), code, gate_code, int(bool(log_gate)), B, D,
-                                 D // G if G else 1, x.data_ptr(), gate.data_ptr(), state.data_ptr(),
-                                 new_state.data_ptr(), y.data_ptr(), x.stride(0), gate.stride(0), state.stride(0),
-                                 new_state.stride(0), y.stride(0))
-        _check(_lib.load().tfft_scan_step(args, torch.cuda.current_stream().cuda_stream))
+            _refuse(f"{who}: state and new_state are float32 tensors [{B}, {D}]")
+    y = _out(who, "out", out, x)
+    rows = []
+    for t in (x, gate, state, new_state, y):
+        b, c = t.stride()
+        if c != 1 and t.shape[1] > 1:
+            _refuse(f"{who}: the values of a row are contiguous")
+        rows.append(b)
+    rc = _lib.load().tfft_scan_step(
+        _lib.SCAN_STEP_ARGS.pack(_lib.SCAN_STEP_ARGS.size, code, gate_code, bool(log_gate), B, D, D // G if G else 1, x.data_ptr(),
+                                 gate.data_ptr(), state.data_ptr(), new_state.data_ptr(), y.data_ptr(), *rows), stream)
+    if rc:
+        _check(rc)
     return y

@@ -9,14 +9,13 @@ include/thunderfft_c.h. No counterpart in the reference, whose twiddles belong t
     q, k = rotate(plan, q, k, positions)                  # q [B, L, H, P], k [B, L, H', P], positions int [B, L] or [L]
     dq, dk = rotate(plan, dq, dk, positions, inverse=True)
 """
-import ctypes
 import math
 
 import torch
 
 from . import _lib
 from .api import _check
-from .recurrence import _FLOATS, _on_stream, _refuse
+from .recurrence import _FLOATS, _placed, _refuse
 
 _PAIRS = {"half": 0, "interleaved": 1}
 
@@ -71,13 +70,6 @@ class RotaryPlan:
         self.turns = torch.tensor(words, dtype=torch.int64).to("cuda" if device is None else device)
 
 
-def _tensor(who, name, t, plan, B, L):
-    if t.dim() != 4 or t.shape[0] != B or t.shape[1] != L:
-        _refuse(f"{who}: {name} is [batch, time, heads, values] = [{B}, {L}, ., .], got {tuple(t.shape)}")
-    if t.shape[3] > 1 and t.stride(3) != 1:
-        _refuse(f"{who}: the values of a head of {name} are contiguous")
-
-
 def rotate(plan, q, k=None, positions=None, pairs="half", inverse=False, first=0, out=None, out_k=None, stream=None):
     """q (and k, by the same positions and in the same launch) rotated: a tensor, or a pair where k is given.
 
@@ -86,9 +78,16 @@ def rotate(plan, q, k=None, positions=None, pairs="half", inverse=False, first=0
     2 i with 2 i + 1. positions: int64 or int32 [B, L] or [L] on the device (negative ones turn backwards); without
     them position t is first + t. inverse: the other way round, which is the gradient of rotate. out, out_k: tensors for the results,
     q and k themselves allowed. Asynchronous on `stream` (default: torch's current stream)."""
-    who = "rotate"
     if not q.is_cuda:
-        _refuse(f"{who} needs device tensors")
+        _refuse("rotate needs device tensors")
+    return _placed(_rotate, q.device, stream, plan, q, k, positions, pairs, inverse, first, out, out_k)
+
+
+_NO_TENSOR = (0,) * 9
+
+
+def _rotate(plan, q, k, positions, pairs, inverse, first, out, out_k, stream):
+    who = "rotate"
     code = _FLOATS.get(q.dtype)
     if code is None:
         _refuse(f"{who}: unsupported element type {q.dtype}", 1)
@@ -96,43 +95,45 @@ def rotate(plan, q, k=None, positions=None, pairs="half", inverse=False, first=0
         _refuse(f"{who}: pairs is 'half' or 'interleaved', not {pairs!r}")
     if q.dim() != 4:
         _refuse(f"{who}: q is [batch, time, heads, values], got {tuple(q.shape)}")
-    B, L, P = q.shape[0], q.shape[1], q.shape[3]
+    B, L, _, P = q.shape
     if plan.size > P:
         _refuse(f"{who}: the plan rotates {plan.size} values, a head has {P}")
     if k is None and out_k is not None:
         _refuse(f"{who}: out_k without k")
+    device = q.device
     for t in (plan.turns, k, positions, out, out_k):
-        if t is not None and t.device != q.device:
-            _refuse(f"{who}: tensors on {q.device} and {t.device}")
+        if t is not None and t.device != device:
+            _refuse(f"{who}: tensors on {device} and {t.device}")
     position_bytes = position_batch = position_time = 0
     if positions is not None:
         if positions.dtype not in (torch.int64, torch.int32):
             _refuse(f"{who}: positions are int64 or int32, not {positions.dtype}")
-        if tuple(positions.shape) not in ((B, L), (L,)):
+        if positions.shape != (B, L) and positions.shape != (L,):
             _refuse(f"{who}: positions {tuple(positions.shape)} are neither [{B}, {L}] nor [{L}]")
         position_bytes = positions.element_size()
         position_batch = positions.stride(0) if positions.dim() == 2 else 0
         position_time = positions.stride(-1)
-    with torch.cuda.device(q.device), _on_stream(q.device, stream):
-        views, results = [], []
-        for name, t, o in (("q", q, out), ("k", k, out_k)):
-            if t is None:
-                views.append(_lib.RotaryView())
-                continue
-            _tensor(who, name, t, plan, B, L)
-            if t.dtype != q.dtype or t.shape[3] != P:
-                _refuse(f"{who}: k has q's type and values per head")
-            if o is None:
-                o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-            elif o.dtype != t.dtype or o.shape != t.shape:
-                _refuse(f"{who}: the result of {name} is a {t.dtype} tensor {tuple(t.shape)}")
-            else:
-                _tensor(who, "the result of " + name, o, plan, B, L)
-            results.append(o)
-            views.append(_lib.RotaryView(t.data_ptr(), o.data_ptr(), t.shape[2], *t.stride()[:3], *o.stride()[:3]))
-        args = _lib.RotaryArgs(ctypes.sizeof(_lib.RotaryArgs), code, _PAIRS[pairs], int(bool(inverse)), B, L, P, plan.size,
-                               plan.magnitude, position_bytes, plan.turns.data_ptr(),
-                               None if positions is None else positions.data_ptr(), position_batch, position_time,
-                               int(first), (_lib.RotaryView * 2)(*views))
-        _check(_lib.load().tfft_rotary(args, torch.cuda.current_stream().cuda_stream))
+    views, results = [], []
+    for t, o in ((q, out), (k, out_k)):
+        if t is None:
+            views += _NO_TENSOR
+            continue
+        if t.dim() != 4 or t.dtype != q.dtype or t.shape[0] != B or t.shape[1] != L or t.shape[3] != P:
+            _refuse(f"{who}: k is a {q.dtype} tensor [{B}, {L}, heads, {P}]")
+        if o is None:
+            o = torch.empty(t.shape, dtype=t.dtype, device=device)
+        elif o.dtype != t.dtype or o.shape != t.shape:
+            _refuse(f"{who}: a result is a {t.dtype} tensor {tuple(t.shape)}")
+        *steps, one = t.stride()
+        *out_steps, out_one = o.stride()
+        if P > 1 and (one != 1 or out_one != 1):
+            _refuse(f"{who}: the values of a head are contiguous")
+        results.append(o)
+        views += (t.data_ptr(), o.data_ptr(), t.shape[2], *steps, *out_steps)
+    rc = _lib.load().tfft_rotary(
+        _lib.ROTARY_ARGS.pack(_lib.ROTARY_ARGS.size, code, _PAIRS[pairs], bool(inverse), B, L, P, plan.size, plan.magnitude,
+                              position_bytes, plan.turns.data_ptr(), 0 if positions is None else positions.data_ptr(),
+                              position_batch, position_time, int(first), *views), stream)
+    if rc:
+        _check(rc)
     return results[0] if k is None else tuple(results)
