@@ -8,7 +8,10 @@ using namespace tfft_seq;
 // The words that chunks hand their states on with, cleared by a kernel of the same call: it may be captured and
 // replayed, and nothing of an earlier call is left in them.
 __global__ __launch_bounds__(256) void clear_words(word* words, long long n) {
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) words[i] = 0;
+  const long long at = 4 * ((long long)blockIdx.x * 256 + threadIdx.x);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (at + i < n) words[at + i] = 0;
 }
 
 template <class T, class G>
@@ -121,7 +124,7 @@ const char* check_plan(const P& p) {
 template <class P>
 void clear(const Chunking& c, const P& p, hipStream_t s) {
   const long long n = c.words();
-  if (n) clear_words<<<(unsigned)(n < 256 * 1024 ? (n + 255) / 256 : 1024), 256, 0, s>>>((word*)p.workspace, n);
+  if (n) clear_words<<<(unsigned)((n + 1023) / 1024), 256, 0, s>>>((word*)p.workspace, n);
 }
 
 unsigned blocks(long long threads) { return (unsigned)((threads + 255) / 256); }

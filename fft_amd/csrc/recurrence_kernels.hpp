@@ -6,11 +6,12 @@
 // workgroups of earlier chunks, and walks its steps once more from there to write the results. The second walk multiplies as
 // the definition does; only the states between pieces come from joined maps.
 //
-// The state travels between workgroups in 64-bit words, the fp32 value below and 1 above, written and read by single
-// relaxed device-scope atomics on words that a kernel of the same call has zeroed: a word with the upper half set is
-// complete, so no fence (on this chip a write-back of the whole L2) is needed. Chunks are taken by a ticket in the order in
-// which they depend on each other: whatever a workgroup waits for has been taken before it by a workgroup that is already
-// running and waits for still earlier ones only, so every wait ends. The order of all sums is fixed by the sizes.
+// States and maps travel between workgroups in single words that a kernel of the same call has zeroed, written and read by
+// relaxed device-scope atomics: (A, B) as two fp32 in 64 bits, a state as one fp32 in 32 bits, a zero among them written as -0.0
+// (in A, where the sign of a zero does not show), so that a word with a bit set is there and complete and no fence (on this chip
+// a write-back of a whole L2) is needed. Workgroups take chunks by tickets, in the order in which chunks depend on each
+// other, one after the other: whoever holds the smallest ticket that is not done waits for nothing that is not there, so
+// every wait ends. The order of all sums is fixed by the sizes.
 #pragma once
 #include "seq_common.hpp"
 
@@ -24,25 +25,38 @@ struct Chunking {
   int waves = 0;         // of a workgroup
   int group = 1;         // chunks whose (A, B) are joined directly; the state behind each group is handed on
   int lanes = 64;        // signals: threads of a row, where a wave holds several rows
-  long long state_words = 0;  // words of one chunk
-  long long words() const {  // the ticket, two words a state and chunk where groups are used, one a state and group
-    return chunks <= 1 ? 0 : 1 + state_words * ((group > 1 ? 2 * chunks : 0) + (chunks + group - 1) / group);
+  long long state_words = 0;  // states of one chunk
+  // 64-bit words: the ticket, a map a state and chunk where groups are used, half a word a state and group
+  long long words() const {
+    return chunks <= 1 ? 0 : 1 + state_words * (group > 1 ? chunks : 0) + (state_words * ((chunks + group - 1) / group) + 1) / 2;
   }
 };
 
-__device__ __forceinline__ void publish(word* at, float v) {
-  __hip_atomic_store(at, (1ull << 32) | __float_as_uint(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+__device__ __forceinline__ void publish_map(word* at, float A, float B) {
+  const unsigned a = __float_as_uint(A);
+  __hip_atomic_store(at, (word)(a ? a : 0x80000000u) << 32 | __float_as_uint(B), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ word peek(const word* at) {
+__device__ __forceinline__ void publish_state(unsigned* at, float h) {
+  const unsigned v = __float_as_uint(h);
+  __hip_atomic_store(at, v ? v : 0x80000000u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <class W>
+__device__ __forceinline__ W peek(const W* at) {
   return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ float await(const word* at) {
-  word w = peek(at);
-  while (!(w >> 32)) {
+template <class W>
+__device__ __forceinline__ W await(const W* at) {
+  W w = peek(at);
+  while (!w) {
     __builtin_amdgcn_s_sleep(1);
     w = peek(at);
   }
-  return __uint_as_float((unsigned)w);
+  return w;
+}
+__device__ __forceinline__ float map_a(word w) { return __uint_as_float((unsigned)(w >> 32)); }
+__device__ __forceinline__ float map_b(word w) { return __uint_as_float((unsigned)w); }
+__device__ __forceinline__ unsigned next_ticket(word* words) {
+  return (unsigned)__hip_atomic_fetch_add(words, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // A h + B; a state of zero stays out of a product that may have overflowed

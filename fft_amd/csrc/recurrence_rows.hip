@@ -11,14 +11,11 @@ namespace {
 // A lane holds a run of V channels of one batch entry over S steps, a wave 64 runs, a workgroup `waves` pieces of S steps one
 // behind the other. Channels are counted over the whole batch (each entry padded to whole runs), so few channels
 // fill a wave too.
-#ifndef FS
-#define FS 16
-#define FW 8
-#define FO 4
-#endif
-constexpr int kSteps = FS, kMaxWaves = FW, kMaxGroup = 16, kResident = 512;
+//
+constexpr int kMaxWaves = 8, kMaxGroup = 16, kResident = 512, kRun = 2;
+constexpr int kStepsForward = 16;
 template <class T>
-constexpr int run_of = 2;
+constexpr int kStepsBackward = sizeof(T) == 4 ? 8 : 16;
 
 // Runs take 32-bit offsets, which the plan has checked; single elements may lie anywhere
 template <int V>
@@ -33,11 +30,13 @@ struct Shape {
   word* words;
 };
 
-// Lane's place: first channel n among the states, batch entry b, channel c, valid channels of the run. first: the batch entry
-// that the tile's addresses start from, the same for all lanes.
+// Lane's place: first channel n among the states, batch entry b, first channel c of its run and how many channels of it are the
+// lane's own. The last run of a row that does not fill it lies over the run before, so that every lane can load whole runs:
+// its own channels are the run's last ones, the others' results are dropped. Lanes behind the last channel have none and lie
+// over the tile's first run. first: the batch entry that the tile's addresses start from, the same for all lanes.
 struct Place {
   unsigned n;
-  int b, c, valid, first;
+  int b, c, own, first;
 };
 template <int V>
 __device__ __forceinline__ Place place_of(const Shape& f, unsigned tile, int lane) {
@@ -48,11 +47,12 @@ __device__ __forceinline__ Place place_of(const Shape& f, unsigned tile, int lan
     p.b = p.n / (unsigned)f.padded;
     p.c = p.n - p.b * (unsigned)f.padded;
   } else {
-    p.first = p.b = tile / f.tiles_of_entry;
+    p.first = p.b = __builtin_amdgcn_readfirstlane(tile / f.tiles_of_entry);
     p.c = (tile - p.b * f.tiles_of_entry) * (64 * V) + lane * V;
   }
-  p.valid = p.b >= f.batch || p.c >= f.channels ? 0 : min(V, f.channels - p.c);
-  if (p.valid == 0) p.b = p.first, p.c = 0;
+  p.own = p.b >= f.batch || p.c >= f.channels ? 0 : min(V, f.channels - p.c);
+  if (p.own == 0) p.b = p.first, p.c = 0;
+  else p.c -= V - p.own;
   return p;
 }
 
@@ -67,177 +67,232 @@ struct Lane {
       : base((char*)v.data + p.first * v.batch * (long long)sizeof(T)),
         off((Off)(((p.b - p.first) * v.batch + c * v.channel) * (long long)sizeof(T))),
         step(v.time * (long long)sizeof(T)) {}
+  // the lane's address at step t (the same for the wave), and its move to the next or the previous step: an addition in scalar
+  // registers, said so for the compiler, which otherwise holds an address a step
+  __device__ __forceinline__ void go(int t) {
+    const uint64_t b = (uint64_t)(base + t * step);
+    base = (char*)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32 |
+                   (uint32_t)__builtin_amdgcn_readfirstlane((int)b));
+  }
+  __device__ __forceinline__ void move(long long by) {
+    base += by;
+    asm("" : "+s"(base));
+  }
   __device__ __forceinline__ T* at(int t) const { return (T*)(base + t * step + off); }
+  __device__ __forceinline__ T* here() const { return (T*)(base + off); }
 };
-
-// What ran before this chunk: the state at its start, from the words of earlier chunks. Called by all threads of a workgroup
-// with the (A, B) of its whole chunk in the last wave. Publishes this chunk's own words on the way.
-template <int V>
-struct Lookback {
-  float A[kMaxGroup][64 * V], B[kMaxGroup][64 * V], h[64 * V];
-};
-template <int V>
-__device__ __forceinline__ void state_before(const Shape& f, Lookback<V>& lds, unsigned chunk, long long n, int wave, int waves,
-                                             int lane, const float (&A)[V], const float (&B)[V], float (&h)[V]) {
-  // h comes in as the state before the first chunk
-  if (f.chunks <= 1) return;
-  word* parts = f.words + 1;
-  word* states = parts + (f.group > 1 ? 2 * f.state_words * f.chunks : 0);
-  const int r = chunk % f.group, q = chunk / f.group;
-  const bool last = wave == waves - 1, more = chunk + 1 < (unsigned)f.chunks;
-  if (f.group > 1) {
-    if (last && more && r != f.group - 1) {
-      word* own = parts + 2 * f.state_words * chunk + n;
-#pragma unroll
-      for (int v = 0; v < V; ++v) publish(own + v, A[v]), publish(own + f.state_words + v, B[v]);
-    }
-    for (int k = wave; k < r; k += waves) {
-      const word* from = parts + 2 * f.state_words * (chunk - r + k) + n;
-      float a[V], b[V];
-#pragma unroll
-      for (int v = 0; v < V; ++v) a[v] = await(from + v), b[v] = await(from + f.state_words + v);
-#pragma unroll
-      for (int v = 0; v < V; ++v) lds.A[k][lane * V + v] = a[v], lds.B[k][lane * V + v] = b[v];
-    }
-  }
-  if (last) {
-    if (q > 0) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) h[v] = await(states + f.state_words * (q - 1) + n + v);
-    }
-    if (f.group == 1 && more) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) publish(states + f.state_words * q + n + v, join(A[v], h[v], B[v]));
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v) lds.h[lane * V + v] = h[v];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int v = 0; v < V; ++v) h[v] = lds.h[lane * V + v];
-  for (int k = 0; k < r; ++k) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = join(lds.A[k][lane * V + v], h[v], lds.B[k][lane * V + v]);
-  }
-  if (f.group > 1 && last && more && r == f.group - 1) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) publish(states + f.state_words * q + n + v, join(A[v], h[v], B[v]));
-  }
-}
-
-// Chunk and tile of this workgroup: a ticket where chunks depend on each other
-__device__ __forceinline__ unsigned take(const Shape& f, unsigned* ticket) {
-  if (f.chunks <= 1) return blockIdx.x;
-  if (threadIdx.x == 0) *ticket = (unsigned)__hip_atomic_fetch_add(f.words, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
-  return __builtin_amdgcn_readfirstlane(*ticket);
-}
-
-// The (A, B) in front of each wave's piece, and behind the last wave's the chunk's
-template <int V>
-struct Pieces {
-  float A[kMaxWaves][64 * V], B[kMaxWaves][64 * V];
-};
-template <int V>
-__device__ __forceinline__ void join_pieces(Pieces<V>& lds, int wave, int waves, int lane, const float (&A)[V], const float (&B)[V],
-                                            float (&front_a)[V], float (&front_b)[V], float (&chunk_a)[V], float (&chunk_b)[V]) {
-#pragma unroll
-  for (int v = 0; v < V; ++v) lds.A[wave][lane * V + v] = A[v], lds.B[wave][lane * V + v] = B[v];
-  __syncthreads();
-#pragma unroll
-  for (int v = 0; v < V; ++v) front_a[v] = 1.0f, front_b[v] = 0.0f;
-  for (int w = 0; w < wave; ++w) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const float a = lds.A[w][lane * V + v];
-      front_b[v] = join(a, front_b[v], lds.B[w][lane * V + v]);
-      front_a[v] *= a;
-    }
-  }
-#pragma unroll
-  for (int v = 0; v < V; ++v) chunk_a[v] = front_a[v] * A[v], chunk_b[v] = join(A[v], front_b[v], B[v]);
-}
-
-// Decays of S steps of a lane, one for the run (VG = 1) or one a channel; 1 behind the sequence
-template <int S, int VG, class G, class Off>
-__device__ __forceinline__ void load_decays(const Lane<G, Off>& g, int t0, int len, int valid, int log_gate, float (&a)[S][VG]) {
-  const int vg = min(valid, VG);
-  if (__all(t0 + S <= len && vg == VG)) {
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-      const Run<G, VG> r = load_run<G, VG>(g.at(t0 + s));
-#pragma unroll
-      for (int v = 0; v < VG; ++v) a[s][v] = r.get(v);
-    }
-  } else {
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-#pragma unroll
-      for (int v = 0; v < VG; ++v) a[s][v] = log_gate ? 0.0f : 1.0f;
-      if (t0 + s < len && vg > 0) {
-        const Run<G, VG> r = load_some<VG>(g.at(t0 + s), vg);
-#pragma unroll
-        for (int v = 0; v < VG; ++v) a[s][v] = r.get(v);
-      }
-    }
-  }
-  if (log_gate) {
-#pragma unroll
-    for (int s = 0; s < S; ++s)
-#pragma unroll
-      for (int v = 0; v < VG; ++v) a[s][v] = exp_decay(a[s][v]);
-  }
-}
-
-// Values of the same steps; 0 outside the sequence
-template <int S, int V, class T, class Off>
-__device__ __forceinline__ void load_values(const Lane<T, Off>& x, int t0, int len, int valid, Run<T, V> (&r)[S]) {
-  if (__all(t0 >= 0 && t0 + S <= len && valid == V)) {
-#pragma unroll
-    for (int s = 0; s < S; ++s) r[s] = load_run<T, V>(x.at(t0 + s));
-  } else {
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-      r[s].clear();
-      if (t0 + s >= 0 && t0 + s < len && valid > 0) r[s] = load_some<V>(x.at(t0 + s), valid);
-    }
-  }
-}
 
 template <int V>
 __device__ __forceinline__ void load_state(const float* from, const Place& p, int channels, float (&h)[V]) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) h[v] = from && v < p.valid ? from[(long long)p.b * channels + p.c + v] : 0.0f;
+  for (int v = 0; v < V; ++v) h[v] = from && v >= V - p.own ? from[(long long)p.b * channels + p.c + v] : 0.0f;
 }
 template <int V>
 __device__ __forceinline__ void store_state(float* to, const Place& p, int channels, const float (&h)[V]) {
   if (!to) return;
 #pragma unroll
   for (int v = 0; v < V; ++v)
-    if (v < p.valid) to[(long long)p.b * channels + p.c + v] = h[v];
+    if (v >= V - p.own) to[(long long)p.b * channels + p.c + v] = h[v];
+}
+
+// The state in front of this chunk, for the wave that has the (A, B) of the whole chunk, from the words of earlier chunks (or
+// `start`, in front of the first). Publishes this chunk's own words on the way. The maps of the group are joined while the state
+// behind the group before is still on its way, so that it is handed on at once when it comes.
+template <int V>
+__device__ __forceinline__ void state_before(const Shape& f, const float* start, const Place& at, unsigned chunk, const float (&A)[V],
+                                             const float (&B)[V], float (&h)[V]) {
+  word* maps = f.words + 1;
+  unsigned* states = (unsigned*)(maps + (f.group > 1 ? f.state_words * f.chunks : 0));
+  const int r = chunk % f.group, q = chunk / f.group;
+  const bool more = chunk + 1 < (unsigned)f.chunks;
+  if (more && r != f.group - 1) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) publish_map(maps + f.state_words * chunk + at.n + v, A[v], B[v]);
+  }
+  float a[V], b[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) a[v] = 1.0f, b[v] = 0.0f;
+  constexpr int kAtOnce = 4;
+#pragma unroll 1
+  for (int k = 0; k < r; k += kAtOnce) {
+    word w[kAtOnce][V];
+    const word* from = maps + f.state_words * (chunk - r + k) + at.n;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i)
+#pragma unroll
+      for (int v = 0; v < V; ++v) w[i][v] = peek(from + (k + i < r ? f.state_words * i : 0) + v);
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (k + i >= r) break;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if (!w[i][v]) w[i][v] = await(from + f.state_words * i + v);
+        b[v] = join(map_a(w[i][v]), b[v], map_b(w[i][v]));
+        a[v] *= map_a(w[i][v]);
+      }
+    }
+  }
+  if (q == 0) {
+    load_state<V>(start, at, f.channels, h);
+  } else {
+    unsigned w[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) w[v] = peek(states + f.state_words * (q - 1) + at.n + v);
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = __uint_as_float(w[v] ? w[v] : await(states + f.state_words * (q - 1) + at.n + v));
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) h[v] = join(a[v], h[v], b[v]);
+  if (more && r == f.group - 1) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) publish_state(states + f.state_words * q + at.n + v, join(A[v], h[v], B[v]));
+  }
+}
+
+// The (A, B) of the waves' pieces, the state in front of the chunk, the ticket
+template <int V>
+struct Joint {
+  float A[kMaxWaves][64 * V], B[kMaxWaves][64 * V], h[64 * V];
+  unsigned ticket;
+};
+// those in front of this wave's piece
+template <int V>
+__device__ __forceinline__ void join_pieces(const Joint<V>& lds, int wave, int lane, float (&a)[V], float (&b)[V]) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) a[v] = 1.0f, b[v] = 0.0f;
+#pragma unroll 2
+  for (int w = 0; w < wave; ++w) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float A = lds.A[w][lane * V + v];
+      b[v] = join(A, b[v], lds.B[w][lane * V + v]);
+      a[v] *= A;
+    }
+  }
+}
+
+// Asks for V elements at each of S steps from t0 on. Steps in front of the first and behind the last are asked for there (what
+// that gives is not used): one path for all, because a load whose register two paths could have filled is waited for where they meet.
+template <int S, int V, class T, class Off>
+__device__ __forceinline__ void ask(Lane<T, Off> x, int t0, int last, Run<T, V> (&r)[S]) {
+  x.go(min(max(t0, 0), last));
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    r[s] = load_run<T, V>(x.here());
+    if (s + 1 < S) x.move(t0 + s >= 0 && t0 + s < last ? x.step : 0);
+  }
+}
+// The last step that a wave has use for: a step behind the longest of its sequences is of none
+__device__ __forceinline__ int last_step(const Shape& f, const int* lengths, int len) {
+  if (!lengths) return f.length - 1;
+  for (int m = 1; m < 64; m *= 2) len = max(len, __shfl_xor(len, m));
+  return max(__builtin_amdgcn_readfirstlane(len), 1) - 1;
+}
+
+// What was asked for, with zeros outside the sequence. The values stay two to a register between the two walks: without stay() the
+// compiler holds the first walk's unpacked copies for the second, twice the registers.
+template <int S, int V, class T>
+__device__ __forceinline__ void stay(Run<T, V> (&x)[S]) {
+#pragma unroll
+  for (int s = 0; s < S; ++s)
+#pragma unroll
+    for (uint32_t& w : x[s].w) asm("" : "+v"(w));
+}
+template <int S, int V, class T>
+__device__ __forceinline__ void take(Run<T, V> (&x)[S], int t0, int len, bool all) {
+  if (!all) {
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+      if (t0 + s < 0 || t0 + s >= len) x[s].clear();
+  }
+  stay<S, V>(x);
+}
+template <int S, int V, class G>
+__device__ __forceinline__ void take_decays(const Run<G, V> (&r)[S], int t0, int len, bool all, int log_gate, float (&a)[S][V]) {
+#pragma unroll
+  for (int s = 0; s < S; ++s)
+#pragma unroll
+    for (int v = 0; v < V; ++v) a[s][v] = r[s].get(v);
+  if (log_gate) {
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int v = 0; v < V; ++v) a[s][v] = exp_decay(a[s][v]);
+  }
+  if (!all) {
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int v = 0; v < V; ++v) a[s][v] = t0 + s < len ? a[s][v] : 1.0f;
+  }
+}
+// The lane's own elements of a run
+template <int V, class T>
+__device__ __forceinline__ void put(T* to, const Run<T, V>& r, int own) {
+  if (own == V) return store_run<T, V>(to, r);
+#pragma unroll
+  for (int v = 1; v < V; ++v)
+    if (v >= V - own) {
+      Run<T, 1> one;
+      if constexpr (sizeof(T) == 4) one.w[0] = r.w[v];
+      else one.w[0] = r.w[v / 2] >> (v % 2 * 16);
+      store_run<T, 1>(to + v, one);
+    }
+}
+
+// Chunk and tile of this workgroup: its ticket's where chunks depend on each other
+template <int V>
+__device__ __forceinline__ unsigned turn_of(const Shape& f, Joint<V>& lds) {
+  if (f.chunks <= 1) return blockIdx.x;
+  if (threadIdx.x == 0) lds.ticket = next_ticket(f.words);
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(lds.ticket);
+}
+
+// From the (A, B) of this wave's piece to the state in front of it
+template <int V>
+__device__ __forceinline__ void state_of_piece(const Shape& f, Joint<V>& lds, const float* start, const Place& at, unsigned chunk, int wave,
+                                               int waves, int lane, const float (&A)[V], const float (&B)[V], float (&h)[V]) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) lds.A[wave][lane * V + v] = A[v], lds.B[wave][lane * V + v] = B[v];
+  __syncthreads();
+  float front_a[V], front_b[V];
+  join_pieces<V>(lds, wave, lane, front_a, front_b);
+  if (wave == waves - 1) {
+    float chunk_a[V], chunk_b[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) chunk_a[v] = A[v] * front_a[v], chunk_b[v] = join(A[v], front_b[v], B[v]);
+    state_before<V>(f, start, at, chunk, chunk_a, chunk_b, h);
+#pragma unroll
+    for (int v = 0; v < V; ++v) lds.h[lane * V + v] = h[v];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int v = 0; v < V; ++v) h[v] = join(front_a[v], lds.h[lane * V + v], front_b[v]);
 }
 
 template <class T, class G, int V, int VG>
-__global__ __launch_bounds__(64 * kMaxWaves, FO) void scan_rows_fwd(tfft_scan_args p, Shape f) {
-  constexpr int S = kSteps;
-  __shared__ Pieces<V> pieces;
-  __shared__ Lookback<V> lookback;
-  __shared__ unsigned ticket;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  const unsigned turn = take(f, &ticket), chunk = turn / f.tiles, tile = turn - chunk * f.tiles;
-  const Place at = place_of<V>(f, tile, lane);
-  const int len = steps_of(p.lengths, at.b, f.length), t0 = (int)(chunk * waves + wave) * S;
+__global__ __launch_bounds__(64 * kMaxWaves, 4) void scan_rows_fwd(tfft_scan_args p, Shape f) {
+  constexpr int S = kStepsForward;
   using Off = offset_of<V>;
-  const Lane<T, Off> x(p.x, at, at.c), y(p.y, at, at.c);
-  const Lane<G, Off> g(p.gate, at, f.share == 1 ? at.c : at.c / f.share);
+  __shared__ Joint<V> lds;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const unsigned turn = turn_of<V>(f, lds), chunk = __builtin_amdgcn_readfirstlane(turn / f.tiles);
+  const Place at = place_of<V>(f, turn - chunk * f.tiles, lane);
+  const int len = steps_of(p.lengths, at.b, f.length), t0 = (int)(chunk * waves + wave) * S;
+  const bool all = __all(t0 + S <= len && at.own == V);
+  Run<T, V> x[S];
+  Run<G, VG> g[S];
+  if (f.length > 0) {
+    const int last = last_step(f, p.lengths, len);
+    ask<S, V>(Lane<T, Off>(p.x, at, at.c), t0, last, x);
+    ask<S, VG>(Lane<G, Off>(p.gate, at, f.share == 1 ? at.c : at.c / f.share), t0, last, g);
+  }
   float a[S][VG];
-  Run<T, V> xr[S];
-  load_values<S, V>(x, t0, len, at.valid, xr);
-  load_decays<S, VG>(g, t0, len, at.valid, f.log_gate, a);
-  float h[V];
-  load_state<V>(p.initial, at, f.channels, h);
+  take<S, V>(x, t0, len, all);
+  take_decays<S, VG>(g, t0, len, all, f.log_gate, a);
 
-  float A[V], B[V], front_a[V], front_b[V], chunk_a[V], chunk_b[V];
+  float A[V], B[V], h[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) A[v] = 1.0f, B[v] = 0.0f;
 #pragma unroll
@@ -245,65 +300,80 @@ __global__ __launch_bounds__(64 * kMaxWaves, FO) void scan_rows_fwd(tfft_scan_ar
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       A[v] *= a[s][v % VG];
-      B[v] = fmaf(a[s][v % VG], B[v], xr[s].get(v));
+      B[v] = fmaf(a[s][v % VG], B[v], x[s].get(v));
     }
-  join_pieces<V>(pieces, wave, waves, lane, A, B, front_a, front_b, chunk_a, chunk_b);
-  state_before<V>(f, lookback, chunk, at.n, wave, waves, lane, chunk_a, chunk_b, h);
-#pragma unroll
-  for (int v = 0; v < V; ++v) h[v] = join(front_a[v], h[v], front_b[v]);
+  stay<S, V>(x);
+  state_of_piece<V>(f, lds, p.initial, at, chunk, wave, waves, lane, A, B, h);
 
-  if (__all(t0 + S <= len && at.valid == V)) {
+  Lane<T, Off> y(p.y, at, at.c);
+  y.go(t0);
+  const auto walk = [&](auto whole) {
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
+    for (int s = 0; s < S; ++s, y.move(y.step)) {
       Run<T, V> r;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        h[v] = fmaf(a[s][v % VG], h[v], xr[s].get(v));
-        r.set(v, h[v]);
+        h[v] = fmaf(a[s][v % VG], h[v], x[s].get(v));
+        r.set(v, whole.value || t0 + s < len ? h[v] : 0.0f);
       }
-      store_run<T, V>(y.at(t0 + s), r);
+      if (whole.value || t0 + s < f.length) put<V>(y.here(), r, whole.value ? V : at.own);
     }
-  } else {
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-      Run<T, V> r;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        h[v] = fmaf(a[s][v % VG], h[v], xr[s].get(v));
-        r.set(v, t0 + s < len ? h[v] : 0.0f);
-      }
-      if (t0 + s < f.length) store_some<V>(y.at(t0 + s), r, at.valid);
-    }
-  }
+  };
+  if (all) walk(std::true_type());
+  else walk(std::false_type());
   if (chunk + 1 == (unsigned)f.chunks && wave == waves - 1) store_state<V>(p.last, at, f.channels, h);
+}
+
+// Sums of N values over groups of `lanes` lanes (a power of two, at least N), one value a lane: every exchange halves the
+// values that a lane still has, N - 1 exchanges where one sum after the other takes N times the logarithm. The lane
+// ends with the sum of value `at`. M: how far apart the lanes of the next exchange lie.
+template <int N, int M = 1>
+__device__ __forceinline__ float sum_values(const float (&q)[N], int lane, int lanes, int& at) {
+  if constexpr (N == 1) {
+    float sum = q[0];
+    for (int m = M; m < lanes; m *= 2) sum += __shfl_xor(sum, m);
+    return sum;
+  } else {
+    const bool upper = lane & M;
+    at = 2 * at + upper;
+    float half[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const float keep = upper ? q[i + N / 2] : q[i], give = upper ? q[i] : q[i + N / 2];
+      half[i] = keep + __shfl_xor(give, M);
+    }
+    return sum_values<N / 2, 2 * M>(half, lane, lanes, at);
+  }
 }
 
 // Backwards in time: chunk 0 is the latest, wave 0 has the latest piece. `lanes`: lanes that share a gate, 0 where each
 // channel's term goes to `parts` (fp32 [batch][time][channel]) to be summed by a kernel behind.
 template <class T, class G, int V, int VG>
-__global__ __launch_bounds__(64 * kMaxWaves, FO) void scan_rows_bwd(tfft_scan_grad_args p, Shape f, float* parts, int lanes) {
-  constexpr int S = kSteps;
-  __shared__ Pieces<V> pieces;
-  __shared__ Lookback<V> lookback;
-  __shared__ unsigned ticket;
+__global__ __launch_bounds__(64 * kMaxWaves, 4) void scan_rows_bwd(tfft_scan_grad_args p, Shape f, float* parts, int lanes) {
+  constexpr int S = kStepsBackward<T>;
+  constexpr bool kShared = V == 1 || VG < V;  // a gate may have several channels
+  using Off = offset_of<V>;
+  __shared__ Joint<V> lds;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  const unsigned turn = take(f, &ticket), chunk = turn / f.tiles, tile = turn - chunk * f.tiles;
-  const Place at = place_of<V>(f, tile, lane);
+  const unsigned turn = turn_of<V>(f, lds), chunk = __builtin_amdgcn_readfirstlane(turn / f.tiles);
+  const Place at = place_of<V>(f, turn - chunk * f.tiles, lane);
   const int len = steps_of(p.lengths, at.b, f.length);
   const int t0 = ((int)(f.chunks - 1 - chunk) * waves + (waves - 1 - wave)) * S;
-  using Off = offset_of<V>;
+  const bool all = __all(t0 + S <= len && at.own == V);
   const int gate = f.share == 1 ? at.c : at.c / f.share;
-  const Lane<T, Off> dy(p.dy, at, at.c), y(p.y, at, at.c), dx(p.dx, at, at.c);
-  const Lane<G, Off> g(p.gate, at, gate), dg(p.dgate, at, gate);
-  float a[S][VG];
   Run<T, V> d[S], before[S];
-  load_values<S, V>(dy, t0, len, at.valid, d);
-  load_decays<S, VG>(g, t0, len, at.valid, f.log_gate, a);
-  load_values<S, V>(y, t0 - 1, len, at.valid, before);
-  float c[V];
-  load_state<V>(p.dlast, at, f.channels, c);
+  Run<G, VG> g[S];
+  if (f.length > 0) {
+    const int last = last_step(f, p.lengths, len);
+    ask<S, V>(Lane<T, Off>(p.dy, at, at.c), t0, last, d);
+    ask<S, VG>(Lane<G, Off>(p.gate, at, gate), t0, last, g);
+    ask<S, V>(Lane<T, Off>(p.y, at, at.c), t0 - 1, last, before);
+  }
+  float a[S][VG];
+  take<S, V>(d, t0, len, all);
+  take_decays<S, VG>(g, t0, len, all, f.log_gate, a);
 
-  float A[V], B[V], front_a[V], front_b[V], chunk_a[V], chunk_b[V];
+  float A[V], B[V], c[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) A[v] = 1.0f, B[v] = 0.0f;
 #pragma unroll
@@ -313,16 +383,21 @@ __global__ __launch_bounds__(64 * kMaxWaves, FO) void scan_rows_bwd(tfft_scan_gr
       A[v] *= a[s][v % VG];
       B[v] = a[s][v % VG] * (B[v] + d[s].get(v));
     }
-  join_pieces<V>(pieces, wave, waves, lane, A, B, front_a, front_b, chunk_a, chunk_b);
-  state_before<V>(f, lookback, chunk, at.n, wave, waves, lane, chunk_a, chunk_b, c);
-#pragma unroll
-  for (int v = 0; v < V; ++v) c[v] = join(front_a[v], c[v], front_b[v]);
+  stay<S, V>(d);
+  state_of_piece<V>(f, lds, p.dlast, at, chunk, wave, waves, lane, A, B, c);
 
+  take<S, V>(before, t0 - 1, len, all && t0 > 0);
   float start[V];
-  load_state<V>(p.initial, at, f.channels, start);
+#pragma unroll
+  for (int v = 0; v < V; ++v) start[v] = 0.0f;
+  if (t0 == 0) load_state<V>(p.initial, at, f.channels, start);
+  Lane<T, Off> dx(p.dx, at, at.c);
+  Lane<G, Off> dg(p.dgate, at, gate);
+  dx.go(t0 + S - 1), dg.go(t0 + S - 1);
+  float sums[S];  // of the run, where a gate has one or more runs of channels
   const auto walk = [&](auto whole) {
 #pragma unroll
-    for (int s = S - 1; s >= 0; --s) {
+    for (int s = S - 1; s >= 0; --s, dx.move(-dx.step), dg.move(-dg.step)) {
       const int t = t0 + s;
       Run<T, V> r;
       float da[V];
@@ -337,32 +412,42 @@ __global__ __launch_bounds__(64 * kMaxWaves, FO) void scan_rows_bwd(tfft_scan_gr
         if (!whole.value) da[v] = t < len ? da[v] : 0.0f;
       }
       const bool in = whole.value || t < f.length;
-      const int valid = whole.value ? V : at.valid;
-      if (in) store_some<V>(dx.at(t), r, valid);
-      if (f.share == 1) {
+      const int own = whole.value ? V : at.own;
+      if (in) put<V>(dx.here(), r, own);
+      if (!kShared || (V == 1 && f.share == 1)) {
         Run<G, V> q;
 #pragma unroll
         for (int v = 0; v < V; ++v) q.set(v, da[v]);
-        if (in) store_some<V>(dg.at(t), q, valid);
+        if (in) put<V>(dg.here(), q, own);
       } else if (lanes > 0) {
-        float sum = da[0];
+        sums[s] = da[0];
 #pragma unroll
-        for (int v = 1; v < V; ++v) sum += da[v];
-        for (int m = 1; m < lanes; m *= 2) sum += __shfl_xor(sum, m);
-        if (in && valid > 0 && (lane & (lanes - 1)) == 0) {
-          Run<G, 1> q;
-          q.set(0, sum);
-          store_run<G, 1>(dg.at(t), q);
-        }
+        for (int v = 1; v < V; ++v) sums[s] += da[v];
       } else if (in) {
 #pragma unroll
         for (int v = 0; v < V; ++v)
-          if (v < valid) parts[((long long)at.b * f.length + t) * f.channels + at.c + v] = da[v];
+          if (v >= V - own) parts[((long long)at.b * f.length + t) * f.channels + at.c + v] = da[v];
       }
     }
   };
-  if (__all(t0 + S <= len && at.valid == V)) walk(std::true_type());
+  if (all) walk(std::true_type());
   else walk(std::false_type());
+  if (kShared && f.share > 1) {
+    if (lanes >= S) {
+      int s = 0;
+      Run<G, 1> q;
+      q.set(0, sum_values<S>(sums, lane, lanes, s));
+      if (at.own > 0 && (lane & (lanes - 1)) < S && t0 + s < f.length) store_run<G, 1>(Lane<G, long long>(p.dgate, at, gate).at(t0 + s), q);
+    } else if (lanes > 0) {
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        for (int m = 1; m < lanes; m *= 2) sums[s] += __shfl_xor(sums[s], m);
+        Run<G, 1> q;
+        q.set(0, sums[s]);
+        if (at.own > 0 && (lane & (lanes - 1)) == 0 && t0 + s < f.length) store_run<G, 1>(Lane<G, long long>(p.dgate, at, gate).at(t0 + s), q);
+      }
+    }
+  }
   if (chunk + 1 == (unsigned)f.chunks && wave == waves - 1) store_state<V>(p.dinitial, at, f.channels, c);
 }
 
@@ -378,7 +463,7 @@ __global__ __launch_bounds__(256) void sum_shares(tfft_scan_grad_args p, const f
   ((G*)p.dgate.data)[b * p.dgate.batch + t * p.dgate.time + g * p.dgate.channel] = from_f32<G>(sum);
 }
 
-int run_length(int dtype) { return dtype == TFFT_F32 ? run_of<float> : run_of<f16>; }
+int steps_backward(int dtype) { return dtype == TFFT_F32 ? kStepsBackward<float> : kStepsBackward<f16>; }
 
 // Tiles run through the whole batch where that keeps a lane's offsets within 32 bits, so that few channels fill a wave too; else
 // each batch entry has tiles of its own.
@@ -389,8 +474,7 @@ bool through_batch(int run, long long batch, long long channels, std::initialize
   return true;
 }
 
-Chunking plan(long long batch, long long length, long long channels, int run, bool through) {
-  constexpr int steps = kSteps;
+Chunking plan(long long batch, long long length, long long channels, int run, bool through, int steps) {
   Chunking c;
   const long long padded = (channels + run - 1) / run * run, width = 64 * run;
   c.tiles = through ? (batch * padded + width - 1) / width : batch * ((channels + width - 1) / width);
@@ -418,23 +502,27 @@ bool gate_fits(const tfft_seq_view& gate, long long share, int run) { return sha
 }  // namespace
 
 bool rows_vector(const tfft_scan_args& p) {
-  return p.x.channel == 1 && p.y.channel == 1 && gate_fits(p.gate, p.share, run_length(p.dtype));
+  return p.channels >= kRun && p.x.channel == 1 && p.y.channel == 1 && gate_fits(p.gate, p.share, kRun);
 }
 bool rows_vector(const tfft_scan_grad_args& p) {
-  return p.dy.channel == 1 && p.y.channel == 1 && p.dx.channel == 1 && gate_fits(p.gate, p.share, run_length(p.dtype)) &&
+  return p.channels >= kRun && p.dy.channel == 1 && p.y.channel == 1 && p.dx.channel == 1 && gate_fits(p.gate, p.share, kRun) &&
          (p.share > 1 || p.dgate.channel == 1);
 }
 
-static int run_of_call(const tfft_scan_args& p) { return rows_vector(p) ? run_length(p.dtype) : 1; }
-static int run_of_call(const tfft_scan_grad_args& p) { return rows_vector(p) ? run_length(p.dtype) : 1; }
+static int run_of_call(const tfft_scan_args& p) { return rows_vector(p) ? kRun : 1; }
+static int run_of_call(const tfft_scan_grad_args& p) { return rows_vector(p) ? kRun : 1; }
 static bool through_batch(const tfft_scan_args& p) {
   return through_batch(run_of_call(p), p.batch, p.channels, {&p.x, &p.gate, &p.y});
 }
 static bool through_batch(const tfft_scan_grad_args& p) {
   return through_batch(run_of_call(p), p.batch, p.channels, {&p.dy, &p.y, &p.gate, &p.dx, &p.dgate});
 }
-Chunking plan_rows(const tfft_scan_args& p) { return plan(p.batch, p.length, p.channels, run_of_call(p), through_batch(p)); }
-Chunking plan_rows(const tfft_scan_grad_args& p) { return plan(p.batch, p.length, p.channels, run_of_call(p), through_batch(p)); }
+Chunking plan_rows(const tfft_scan_args& p) {
+  return plan(p.batch, p.length, p.channels, run_of_call(p), through_batch(p), kStepsForward);
+}
+Chunking plan_rows(const tfft_scan_grad_args& p) {
+  return plan(p.batch, p.length, p.channels, run_of_call(p), through_batch(p), steps_backward(p.dtype));
+}
 
 // Lanes that share a gate, where whole power-of-two groups of a wave's lanes do; 0: summed by a kernel of its own
 static int lanes_of(const tfft_scan_grad_args& p) {
@@ -452,7 +540,7 @@ void launch_rows(const tfft_scan_args& p, const Chunking& c, word* words, hipStr
   with_types(p.dtype, p.gate_dtype, [&](auto t, auto g) {
     using T = decltype(t);
     using G = decltype(g);
-    constexpr int V = run_of<T>;
+    constexpr int V = kRun;
     if (!vector) scan_rows_fwd<T, G, 1, 1><<<grid, block, 0, s>>>(p, f);
     else if (p.share == 1) scan_rows_fwd<T, G, V, V><<<grid, block, 0, s>>>(p, f);
     else scan_rows_fwd<T, G, V, 1><<<grid, block, 0, s>>>(p, f);
@@ -467,7 +555,7 @@ void launch_rows(const tfft_scan_grad_args& p, const Chunking& c, word* words, f
   with_types(p.dtype, p.gate_dtype, [&](auto t, auto g) {
     using T = decltype(t);
     using G = decltype(g);
-    constexpr int V = run_of<T>;
+    constexpr int V = kRun;
     if (!vector) scan_rows_bwd<T, G, 1, 1><<<grid, block, 0, s>>>(p, f, parts, lanes);
     else if (p.share == 1) scan_rows_bwd<T, G, V, V><<<grid, block, 0, s>>>(p, f, parts, lanes);
     else scan_rows_bwd<T, G, V, 1><<<grid, block, 0, s>>>(p, f, parts, lanes);

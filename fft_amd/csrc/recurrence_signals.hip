@@ -84,18 +84,21 @@ __device__ __forceinline__ float state_in_front(const Shape& f, Lds& lds, unsign
     if (wave == waves - 1) {
       const int r = chunk % f.group, q = chunk / f.group;
       const bool more = chunk + 1 < (unsigned)f.chunks;
-      word* own = f.words + 1 + 2 * (row * f.chunks + chunk);
-      word* states = f.words + 1 + 2 * f.rows * f.chunks + row * ((f.chunks + f.group - 1) / f.group);
+      word* own = f.words + 1 + row * f.chunks + chunk;
+      unsigned* states = (unsigned*)(f.words + 1 + f.rows * f.chunks) + row * ((f.chunks + f.group - 1) / f.group);
       const float chunk_a = wave_a * lds.A[wave], chunk_b = join(lds.A[wave], wave_b, lds.B[wave]);
-      if (more && r != f.group - 1 && lane == 0) publish(own, chunk_a), publish(own + 1, chunk_b);
+      if (more && r != f.group - 1 && lane == 0) publish_map(own, chunk_a, chunk_b);
       // lane k joins the k-th chunk of the group, those of this one's past are read together
       float a = 1.0f, b = 0.0f, fa, fb;
-      if (lane < r) a = await(own - 2 * (r - lane)), b = await(own - 2 * (r - lane) + 1);
+      if (lane < r) {
+        const word w = await(own - (r - lane));
+        a = map_a(w), b = map_b(w);
+      }
       scan_lanes(lane, 64, a, b, fa, fb);
       a = __shfl(a, 63), b = __shfl(b, 63);
-      if (q > 0) h = await(states + q - 1);
+      if (q > 0) h = __uint_as_float(await(states + q - 1));
       h = join(a, h, b);
-      if (more && r == f.group - 1 && lane == 0) publish(states + q, join(chunk_a, h, chunk_b));
+      if (more && r == f.group - 1 && lane == 0) publish_state(states + q, join(chunk_a, h, chunk_b));
       if (lane == 0) lds.h = h;
     }
     __syncthreads();
@@ -112,7 +115,7 @@ __device__ __forceinline__ void take(const Shape& f, Lds& lds, long long* row, u
     *row = f.lanes < 64 ? ((long long)blockIdx.x * blockDim.x + threadIdx.x) / f.lanes : (long long)blockIdx.x;
     return;
   }
-  if (threadIdx.x == 0) lds.ticket = (unsigned)__hip_atomic_fetch_add(f.words, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (threadIdx.x == 0) lds.ticket = next_ticket(f.words);
   __syncthreads();
   *chunk = lds.ticket / (unsigned)f.rows;
   *row = lds.ticket % (unsigned)f.rows;
