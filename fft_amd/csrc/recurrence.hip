@@ -118,7 +118,7 @@ const char* check_plan(const P& p) {
   if (p.batch * (p.channels + 3) > kMaxExtent || (p.share > 1 && (__int128)p.batch * p.length * p.channels > ((__int128)1 << 38)))
     return large;
   const Chunking c = plan_of(p);
-  return c.tiles * c.chunks > kMaxExtent ? large : nullptr;
+  return c.blocks() > kMaxExtent ? large : nullptr;
 }
 
 template <class P>

@@ -10,14 +10,22 @@
 // relaxed device-scope atomics: (A, B) as two fp32 in 64 bits, a state as one fp32 in 32 bits, a zero among them written as -0.0
 // (in A, where the sign of a zero does not show), so that a word with a bit set is there and complete and no fence (on this chip
 // a write-back of a whole L2) is needed. Workgroups take chunks by tickets, in the order in which chunks depend on each
-// other, one after the other: whoever holds the smallest ticket that is not done waits for nothing that is not there, so
-// every wait ends. The order of all sums is fixed by the sizes.
+// other: whoever holds the smallest ticket of a counter that is not done waits for nothing that is not there, so every wait
+// ends. The order of all sums is fixed by the sizes.
+//
+// Each of the eight XCDs has a counter of its own, with all chunks of an eighth of the tiles, neighbours beside each other (workgroups
+// go round the XCDs): an XCD then reads whole rows, and lines that two tiles share once. B = 8, L = 4096 with D = 2048: 112 us forward
+// and 184 back, where the XCDs take every eighth tile 116 and 195; with D = 2050 120 and 219 against 140 and 251. With fewer than
+// kManyTiles tiles an eighth is too narrow, and all take from one counter, chunk by chunk: 65537 x 1152 (9 tiles) 129 us against
+// 197 with eight.
 #pragma once
 #include "seq_common.hpp"
 
 namespace tfft_seq {
 
 using word = unsigned long long;
+
+constexpr int kManyTiles = 32, kCounterWords = 16;  // a counter has a cache line of its own
 
 struct Chunking {
   long long tiles = 0;   // rows: groups of channels; signals: groups of rows
@@ -26,11 +34,38 @@ struct Chunking {
   int group = 1;         // chunks whose (A, B) are joined directly; the state behind each group is handed on
   int lanes = 64;        // signals: threads of a row, where a wave holds several rows
   long long state_words = 0;  // states of one chunk
-  // 64-bit words: the ticket, a map a state and chunk where groups are used, half a word a state and group
+  // 64-bit words: the counters, a map a state and chunk where groups are used, half a word a state and group
   long long words() const {
-    return chunks <= 1 ? 0 : 1 + state_words * (group > 1 ? chunks : 0) + (state_words * ((chunks + group - 1) / group) + 1) / 2;
+    return chunks <= 1 ? 0 : kCounterWords * counters() + state_words * (group > 1 ? chunks : 0) +
+                                 (state_words * ((chunks + group - 1) / group) + 1) / 2;
   }
+  int counters() const { return tiles >= kManyTiles ? 8 : 1; }
+  // workgroups; a few find no ticket left where the tiles do not divide evenly
+  long long blocks() const { return chunks <= 1 ? tiles : (tiles + counters() - 1) / counters() * counters() * chunks; }
 };
+
+// Tile and chunk of this workgroup, the same for all threads; false where there is none left. `shared` lies in LDS.
+struct Turns {
+  unsigned tiles, counters, chunks;
+};
+inline Turns turns_of(const Chunking& c) {
+  return Turns{(unsigned)c.tiles, (unsigned)c.counters(), (unsigned)c.chunks};
+}
+__device__ __forceinline__ bool take_turn(const Turns& f, word* words, unsigned* shared, unsigned* tile, unsigned* chunk) {
+  if (f.chunks <= 1) {
+    *tile = blockIdx.x, *chunk = 0;
+    return true;
+  }
+  const unsigned counter = blockIdx.x % f.counters;
+  if (threadIdx.x == 0)
+    *shared = (unsigned)__hip_atomic_fetch_add(words + kCounterWords * counter, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  const unsigned ticket = __builtin_amdgcn_readfirstlane(*shared);
+  const unsigned first = (unsigned)((word)counter * f.tiles / f.counters), mine = (unsigned)((word)(counter + 1) * f.tiles / f.counters) - first;
+  *chunk = __builtin_amdgcn_readfirstlane(ticket / mine);
+  *tile = first + (ticket - *chunk * mine);
+  return *chunk < f.chunks;
+}
 
 __device__ __forceinline__ void publish_map(word* at, float A, float B) {
   const unsigned a = __float_as_uint(A);
@@ -55,10 +90,6 @@ __device__ __forceinline__ W await(const W* at) {
 }
 __device__ __forceinline__ float map_a(word w) { return __uint_as_float((unsigned)(w >> 32)); }
 __device__ __forceinline__ float map_b(word w) { return __uint_as_float((unsigned)w); }
-__device__ __forceinline__ unsigned next_ticket(word* words) {
-  return (unsigned)__hip_atomic_fetch_add(words, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
 // A h + B; a state of zero stays out of a product that may have overflowed
 __device__ __forceinline__ float join(float A, float h, float B) { return h != 0.0f ? fmaf(A, h, B) : B; }
 

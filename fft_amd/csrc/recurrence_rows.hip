@@ -26,7 +26,8 @@ struct Shape {
   int share, log_gate;
   int chunks, group;
   long long state_words;
-  unsigned tiles, tiles_of_entry;  // 0 tiles of an entry: tiles run through the whole batch
+  unsigned tiles_of_entry;  // 0: tiles run through the whole batch
+  Turns turns;
   word* words;
 };
 
@@ -101,7 +102,7 @@ __device__ __forceinline__ void store_state(float* to, const Place& p, int chann
 template <int V>
 __device__ __forceinline__ void state_before(const Shape& f, const float* start, const Place& at, unsigned chunk, const float (&A)[V],
                                              const float (&B)[V], float (&h)[V]) {
-  word* maps = f.words + 1;
+  word* maps = f.words + kCounterWords * f.turns.counters;
   unsigned* states = (unsigned*)(maps + (f.group > 1 ? f.state_words * f.chunks : 0));
   const int r = chunk % f.group, q = chunk / f.group;
   const bool more = chunk + 1 < (unsigned)f.chunks;
@@ -240,15 +241,6 @@ __device__ __forceinline__ void put(T* to, const Run<T, V>& r, int own) {
     }
 }
 
-// Chunk and tile of this workgroup: its ticket's where chunks depend on each other
-template <int V>
-__device__ __forceinline__ unsigned turn_of(const Shape& f, Joint<V>& lds) {
-  if (f.chunks <= 1) return blockIdx.x;
-  if (threadIdx.x == 0) lds.ticket = next_ticket(f.words);
-  __syncthreads();
-  return __builtin_amdgcn_readfirstlane(lds.ticket);
-}
-
 // From the (A, B) of this wave's piece to the state in front of it
 template <int V>
 __device__ __forceinline__ void state_of_piece(const Shape& f, Joint<V>& lds, const float* start, const Place& at, unsigned chunk, int wave,
@@ -277,8 +269,9 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void scan_rows_fwd(tfft_scan_arg
   using Off = offset_of<V>;
   __shared__ Joint<V> lds;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  const unsigned turn = turn_of<V>(f, lds), chunk = __builtin_amdgcn_readfirstlane(turn / f.tiles);
-  const Place at = place_of<V>(f, turn - chunk * f.tiles, lane);
+  unsigned tile, chunk;
+  if (!take_turn(f.turns, f.words, &lds.ticket, &tile, &chunk)) return;
+  const Place at = place_of<V>(f, tile, lane);
   const int len = steps_of(p.lengths, at.b, f.length), t0 = (int)(chunk * waves + wave) * S;
   const bool all = __all(t0 + S <= len && at.own == V);
   Run<T, V> x[S];
@@ -355,8 +348,9 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void scan_rows_bwd(tfft_scan_gra
   using Off = offset_of<V>;
   __shared__ Joint<V> lds;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  const unsigned turn = turn_of<V>(f, lds), chunk = __builtin_amdgcn_readfirstlane(turn / f.tiles);
-  const Place at = place_of<V>(f, turn - chunk * f.tiles, lane);
+  unsigned tile, chunk;
+  if (!take_turn(f.turns, f.words, &lds.ticket, &tile, &chunk)) return;
+  const Place at = place_of<V>(f, tile, lane);
   const int len = steps_of(p.lengths, at.b, f.length);
   const int t0 = ((int)(f.chunks - 1 - chunk) * waves + (waves - 1 - wave)) * S;
   const bool all = __all(t0 + S <= len && at.own == V);
@@ -493,8 +487,7 @@ Chunking plan(long long batch, long long length, long long channels, int run, bo
 template <class P>
 Shape shape_of(const P& p, const Chunking& c, int run, bool through, word* words) {
   return Shape{(int)p.batch, (int)p.length, (int)p.channels, (int)((p.channels + run - 1) / run * run), (int)p.share,
-               p.gate_form == TFFT_GATE_LOG, (int)c.chunks, c.group, c.state_words, (unsigned)c.tiles,
-               through ? 0u : (unsigned)(c.tiles / p.batch), words};
+               p.gate_form == TFFT_GATE_LOG, (int)c.chunks, c.group, c.state_words, through ? 0u : (unsigned)(c.tiles / p.batch), turns_of(c), words};
 }
 
 bool gate_fits(const tfft_seq_view& gate, long long share, int run) { return share == 1 ? gate.channel == 1 : share % run == 0; }
@@ -536,7 +529,7 @@ bool rows_sums_shares(const tfft_scan_grad_args& p) { return p.share > 1 && lane
 void launch_rows(const tfft_scan_args& p, const Chunking& c, word* words, hipStream_t s) {
   const bool vector = rows_vector(p);
   const Shape f = shape_of(p, c, run_of_call(p), through_batch(p), words);
-  const dim3 grid((unsigned)(c.tiles * c.chunks)), block(64 * c.waves);
+  const dim3 grid((unsigned)c.blocks()), block(64 * c.waves);
   with_types(p.dtype, p.gate_dtype, [&](auto t, auto g) {
     using T = decltype(t);
     using G = decltype(g);
@@ -550,7 +543,7 @@ void launch_rows(const tfft_scan_args& p, const Chunking& c, word* words, hipStr
 void launch_rows(const tfft_scan_grad_args& p, const Chunking& c, word* words, float* parts, hipStream_t s) {
   const bool vector = rows_vector(p);
   const Shape f = shape_of(p, c, run_of_call(p), through_batch(p), words);
-  const dim3 grid((unsigned)(c.tiles * c.chunks)), block(64 * c.waves);
+  const dim3 grid((unsigned)c.blocks()), block(64 * c.waves);
   const int lanes = lanes_of(p);
   with_types(p.dtype, p.gate_dtype, [&](auto t, auto g) {
     using T = decltype(t);

@@ -14,36 +14,71 @@ struct Shape {
   long long rows;
   int length, channels, log_gate;
   int chunks, group, lanes;
+  Turns turns;
   word* words;
 };
 
+// Asks for E steps from t0 on. A piece that reaches over the end of the row is asked for as the row's last E steps, so that all
+// threads load whole runs on one path; line_up() then moves its steps to where they belong. Rows shorter than a piece are loaded
+// step by step.
 template <int E, class T>
-__device__ __forceinline__ Run<T, E> load_steps(const T* p, int t0, int len) {
-  return load_some<E>(p + t0, min(max(len - t0, 0), E));
+__device__ __forceinline__ Run<T, E> ask(const T* p, int t0, int length) {
+  if (length < E) return load_some<E>(p, t0 == 0 ? length : 0);
+  return load_run<T, E>(p + max(min(t0, length - E), 0));
+}
+template <int E, class G>
+__device__ __forceinline__ Run<G, E> one(const G* p) {
+  const uint32_t v = load_run<G, 1>(p).w[0];
+  Run<G, E> r;
+#pragma unroll
+  for (uint32_t& w : r.w) w = sizeof(G) == 4 ? v : v | v << 16;
+  return r;
+}
+template <int E, class T>
+__device__ __forceinline__ void line_up(Run<T, E>& r, int t0, int length) {
+  const int by = length < E ? 0 : min(max(t0 - (length - E), 0), E);  // steps that the run starts too early
+  if (__all(by == 0)) return;
+  constexpr int kWords = sizeof(r.w) / 4, kElements = 4 / sizeof(T);
+#pragma unroll
+  for (int m = kWords; m >= 1; m /= 2) {
+    const bool move = by / kElements & m;
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) r.w[i] = move ? (i + m < kWords ? r.w[i + m] : 0u) : r.w[i];
+  }
+  if constexpr (kElements == 2) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) r.w[i] = by & 1 ? r.w[i] >> 16 | (i + 1 < kWords ? r.w[i + 1] << 16 : 0u) : r.w[i];
+  }
 }
 template <int E, class T>
 __device__ __forceinline__ void store_steps(T* p, int t0, int length, const Run<T, E>& r) {
   store_some<E>(p + t0, r, min(max(length - t0, 0), E));
 }
 
-// Decays of E steps; 1 behind the sequence. time is 1, or 0 for one decay throughout.
+// Decays of E steps that were asked for; 1 behind the sequence. time is 1, or 0 for one decay throughout.
 template <int E, class G>
-__device__ __forceinline__ void load_decays(const G* g, long long time, int t0, int len, int log_gate, float (&a)[E]) {
-  if (time) {
-    const Run<G, E> r = load_steps<E>(g, t0, len);
+__device__ __forceinline__ void take_decays(Run<G, E>& r, long long time, int t0, int len, int length, int log_gate, float (&a)[E]) {
+  if (time) line_up<E>(r, t0, length);
 #pragma unroll
-    for (int i = 0; i < E; ++i) a[i] = r.get(i);
-  } else {
-    const float one = t0 < len ? to_f32(g[0]) : 0.0f;
-#pragma unroll
-    for (int i = 0; i < E; ++i) a[i] = one;
-  }
+  for (int i = 0; i < E; ++i) a[i] = r.get(i);
   if (log_gate) {
 #pragma unroll
     for (int i = 0; i < E; ++i) a[i] = exp_decay(a[i]);
   }
+  if (!__all(t0 + E <= len)) {
 #pragma unroll
-  for (int i = 0; i < E; ++i) a[i] = t0 + i < len ? a[i] : 1.0f;
+    for (int i = 0; i < E; ++i) a[i] = t0 + i < len ? a[i] : 1.0f;
+  }
+}
+// Values of E steps that were asked for; 0 from step len - t0 on
+template <int E, class T>
+__device__ __forceinline__ void take(Run<T, E>& r, int t0, int len, int length) {
+  line_up<E>(r, t0, length);
+  if (__all(t0 + E <= len)) return;
+  constexpr int kElements = 4 / sizeof(T);
+#pragma unroll
+  for (int i = 0; i < E; ++i)
+    if (t0 + i >= len) r.w[i / kElements] &= kElements == 1 ? 0u : i % 2 == 0 ? 0xffff0000u : 0x0000ffffu;
 }
 
 // (A, B) of all pieces up to and with this thread's, among `width` threads that follow one another (a power of two,
@@ -84,8 +119,9 @@ __device__ __forceinline__ float state_in_front(const Shape& f, Lds& lds, unsign
     if (wave == waves - 1) {
       const int r = chunk % f.group, q = chunk / f.group;
       const bool more = chunk + 1 < (unsigned)f.chunks;
-      word* own = f.words + 1 + row * f.chunks + chunk;
-      unsigned* states = (unsigned*)(f.words + 1 + f.rows * f.chunks) + row * ((f.chunks + f.group - 1) / f.group);
+      word* maps = f.words + kCounterWords * f.turns.counters;
+      word* own = maps + row * f.chunks + chunk;
+      unsigned* states = (unsigned*)(maps + f.rows * f.chunks) + row * ((f.chunks + f.group - 1) / f.group);
       const float chunk_a = wave_a * lds.A[wave], chunk_b = join(lds.A[wave], wave_b, lds.B[wave]);
       if (more && r != f.group - 1 && lane == 0) publish_map(own, chunk_a, chunk_b);
       // lane k joins the k-th chunk of the group, those of this one's past are read together
@@ -108,17 +144,16 @@ __device__ __forceinline__ float state_in_front(const Shape& f, Lds& lds, unsign
   return join(front_a, h, front_b);
 }
 
-// Row and chunk of this thread; a ticket where chunks depend on each other
-__device__ __forceinline__ void take(const Shape& f, Lds& lds, long long* row, unsigned* chunk) {
-  if (f.chunks <= 1) {
-    *chunk = 0;
-    *row = f.lanes < 64 ? ((long long)blockIdx.x * blockDim.x + threadIdx.x) / f.lanes : (long long)blockIdx.x;
-    return;
+// Row and chunk of this thread
+__device__ __forceinline__ bool take(const Shape& f, Lds& lds, long long* row, unsigned* chunk) {
+  if (f.lanes < 64) {
+    *row = ((long long)blockIdx.x * blockDim.x + threadIdx.x) / f.lanes, *chunk = 0;
+    return true;
   }
-  if (threadIdx.x == 0) lds.ticket = next_ticket(f.words);
-  __syncthreads();
-  *chunk = lds.ticket / (unsigned)f.rows;
-  *row = lds.ticket % (unsigned)f.rows;
+  unsigned tile;
+  const bool there = take_turn(f.turns, f.words, &lds.ticket, &tile, chunk);
+  *row = tile;
+  return there;
 }
 
 template <class T, class G>
@@ -127,7 +162,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void scan_signals_fwd(tfft_scan_arg
   __shared__ Lds lds;
   long long row;
   unsigned chunk;
-  take(f, lds, &row, &chunk);
+  if (!take(f, lds, &row, &chunk)) return;
   const bool live = row < f.rows;
   if (!live) row = 0;
   const int b = (int)(row / f.channels), c = (int)(row % f.channels);
@@ -135,10 +170,17 @@ __global__ __launch_bounds__(64 * kMaxWaves) void scan_signals_fwd(tfft_scan_arg
   const int t0 = (int)(chunk * blockDim.x + piece) * E, len = live ? steps_of(p.lengths, b, f.length) : 0;
   const T* x = (const T*)p.x.data + b * p.x.batch + c * p.x.channel;
   const G* g = (const G*)p.gate.data + b * p.gate.batch + c * p.gate.channel;
-  const Run<T, E> xr = load_steps<E>(x, t0, len);
+  const float initial = p.initial ? p.initial[row] : 0.0f;
+  Run<T, E> xr;
+  Run<G, E> gr;
+  if (f.length > 0) {
+    xr = ask<E>(x, t0, f.length);
+    gr = p.gate.time ? ask<E>(g, t0, f.length) : one<E>(g);
+  }
+  take<E>(xr, t0, len, f.length);
   float a[E];
-  load_decays<E>(g, p.gate.time, t0, len, f.log_gate, a);
-  float h = p.initial ? p.initial[row] : 0.0f;
+  take_decays<E>(gr, p.gate.time, t0, len, f.length, f.log_gate, a);
+  float h = initial;
   float A = 1.0f, B = 0.0f;
 #pragma unroll
   for (int i = 0; i < E; ++i) {
@@ -164,7 +206,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void scan_signals_bwd(tfft_scan_gra
   __shared__ Lds lds;
   long long row;
   unsigned chunk;
-  take(f, lds, &row, &chunk);
+  if (!take(f, lds, &row, &chunk)) return;
   const bool live = row < f.rows;
   if (!live) row = 0;
   const int b = (int)(row / f.channels), c = (int)(row % f.channels);
@@ -174,23 +216,32 @@ __global__ __launch_bounds__(64 * kMaxWaves) void scan_signals_bwd(tfft_scan_gra
   const T* dy = (const T*)p.dy.data + b * p.dy.batch + c * p.dy.channel;
   const T* y = (const T*)p.y.data + b * p.y.batch + c * p.y.channel;
   const G* g = (const G*)p.gate.data + b * p.gate.batch + c * p.gate.channel;
-  const Run<T, E> d = load_steps<E>(dy, t0, len), own = load_steps<E>(y, t0, len);
-  const T before = t0 > 0 && t0 - 1 < len ? y[t0 - 1] : from_f32<T>(0.0f);
+  const float start = p.initial ? p.initial[row] : 0.0f, dlast = p.dlast ? p.dlast[row] : 0.0f;
+  Run<T, E> d, own;
+  Run<T, 1> before;
+  Run<G, E> gr;
+  if (f.length > 0) {
+    d = ask<E>(dy, t0, f.length);
+    gr = p.gate.time ? ask<E>(g, t0, f.length) : one<E>(g);
+    own = ask<E>(y, t0, f.length);
+    before = load_run<T, 1>(y + min(max(t0 - 1, 0), f.length - 1));
+  }
+  take<E>(d, t0, len, f.length);
   float a[E];
-  load_decays<E>(g, p.gate.time, t0, len, f.log_gate, a);
-  const float start = p.initial ? p.initial[row] : 0.0f;
+  take_decays<E>(gr, p.gate.time, t0, len, f.length, f.log_gate, a);
   float A = 1.0f, B = 0.0f;
 #pragma unroll
   for (int i = E - 1; i >= 0; --i) {
     A *= a[i];
     B = a[i] * (B + d.get(i));
   }
-  float k = state_in_front(f, lds, chunk, row, order, A, B, p.dlast ? p.dlast[row] : 0.0f);
+  float k = state_in_front(f, lds, chunk, row, order, A, B, dlast);
+  take<E>(own, t0, len, f.length);
   float dx[E], dgate[E];
 #pragma unroll
   for (int i = E - 1; i >= 0; --i) {
     const float e = d.get(i) + k;
-    const float state = i > 0 ? own.get(i > 0 ? i - 1 : 0) : t0 > 0 ? to_f32(before) : start;
+    const float state = i > 0 ? own.get(i > 0 ? i - 1 : 0) : t0 > 0 ? before.get(0) : start;
     const bool inside = t0 + i < len;
     dgate[i] = inside ? e * state * (f.log_gate ? a[i] : 1.0f) : 0.0f;
     dx[i] = inside ? e : 0.0f;
@@ -228,12 +279,12 @@ Chunking plan(long long batch, long long length, long long channels) {
 template <class P>
 Shape shape_of(const P& p, const Chunking& c, word* words) {
   return Shape{p.batch * p.channels, (int)p.length, (int)p.channels, p.gate_form == TFFT_GATE_LOG,
-               (int)c.chunks, c.group, c.lanes, words};
+               (int)c.chunks, c.group, c.lanes, turns_of(c), words};
 }
 
 dim3 grid_of(const Chunking& c) {
-  const long long per_block = c.lanes < 64 ? 64 * c.waves / c.lanes : 1;
-  return dim3((unsigned)((c.tiles + per_block - 1) / per_block * c.chunks));
+  const long long per_block = 64 * c.waves / c.lanes;
+  return dim3((unsigned)(c.lanes < 64 ? (c.tiles + per_block - 1) / per_block : c.blocks()));
 }
 
 }  // namespace
