@@ -2,6 +2,7 @@
 // at a time, for any other strides.
 #include <initializer_list>
 #include <type_traits>
+#include <utility>
 
 #include "recurrence_kernels.hpp"
 
@@ -174,12 +175,12 @@ __device__ __forceinline__ void join_pieces(const Joint<V>& lds, int wave, int l
 
 // Asks for V elements at each of S steps from t0 on. Steps in front of the first and behind the last are asked for there (what
 // that gives is not used): one path for all, because a load whose register two paths could have filled is waited for where they meet.
-template <int S, int V, class T, class Off>
+template <int S, int V, bool STREAM, class T, class Off>
 __device__ __forceinline__ void ask(Lane<T, Off> x, int t0, int last, Run<T, V> (&r)[S]) {
   x.go(min(max(t0, 0), last));
 #pragma unroll
   for (int s = 0; s < S; ++s) {
-    r[s] = load_run<T, V>(x.here());
+    r[s] = load_run<T, V, STREAM>(x.here());
     if (s + 1 < S) x.move(t0 + s >= 0 && t0 + s < last ? x.step : 0);
   }
 }
@@ -228,9 +229,9 @@ __device__ __forceinline__ void take_decays(const Run<G, V> (&r)[S], int t0, int
   }
 }
 // The lane's own elements of a run
-template <int V, class T>
+template <int V, bool STREAM, class T>
 __device__ __forceinline__ void put(T* to, const Run<T, V>& r, int own) {
-  if (own == V) return store_run<T, V>(to, r);
+  if (own == V) return store_run<T, V, STREAM>(to, r);
 #pragma unroll
   for (int v = 1; v < V; ++v)
     if (v >= V - own) {
@@ -263,7 +264,7 @@ __device__ __forceinline__ void state_of_piece(const Shape& f, Joint<V>& lds, co
   for (int v = 0; v < V; ++v) h[v] = join(front_a[v], lds.h[lane * V + v], front_b[v]);
 }
 
-template <class T, class G, int V, int VG>
+template <class T, class G, int V, int VG, bool STREAM>
 __global__ __launch_bounds__(64 * kMaxWaves, 4) void scan_rows_fwd(tfft_scan_args p, Shape f) {
   constexpr int S = kStepsForward;
   using Off = offset_of<V>;
@@ -278,8 +279,8 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void scan_rows_fwd(tfft_scan_arg
   Run<G, VG> g[S];
   if (f.length > 0) {
     const int last = last_step(f, p.lengths, len);
-    ask<S, V>(Lane<T, Off>(p.x, at, at.c), t0, last, x);
-    ask<S, VG>(Lane<G, Off>(p.gate, at, f.share == 1 ? at.c : at.c / f.share), t0, last, g);
+    ask<S, V, STREAM>(Lane<T, Off>(p.x, at, at.c), t0, last, x);
+    ask<S, VG, STREAM && VG == V>(Lane<G, Off>(p.gate, at, f.share == 1 ? at.c : at.c / f.share), t0, last, g);
   }
   float a[S][VG];
   take<S, V>(x, t0, len, all);
@@ -309,7 +310,7 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void scan_rows_fwd(tfft_scan_arg
         h[v] = fmaf(a[s][v % VG], h[v], x[s].get(v));
         r.set(v, whole.value || t0 + s < len ? h[v] : 0.0f);
       }
-      if (whole.value || t0 + s < f.length) put<V>(y.here(), r, whole.value ? V : at.own);
+      if (whole.value || t0 + s < f.length) put<V, STREAM>(y.here(), r, whole.value ? V : at.own);
     }
   };
   if (all) walk(std::true_type());
@@ -341,7 +342,7 @@ __device__ __forceinline__ float sum_values(const float (&q)[N], int lane, int l
 
 // Backwards in time: chunk 0 is the latest, wave 0 has the latest piece. `lanes`: lanes that share a gate, 0 where each
 // channel's term goes to `parts` (fp32 [batch][time][channel]) to be summed by a kernel behind.
-template <class T, class G, int V, int VG>
+template <class T, class G, int V, int VG, bool STREAM>
 __global__ __launch_bounds__(64 * kMaxWaves, 4) void scan_rows_bwd(tfft_scan_grad_args p, Shape f, float* parts, int lanes) {
   constexpr int S = kStepsBackward<T>;
   constexpr bool kShared = V == 1 || VG < V;  // a gate may have several channels
@@ -359,9 +360,9 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void scan_rows_bwd(tfft_scan_gra
   Run<G, VG> g[S];
   if (f.length > 0) {
     const int last = last_step(f, p.lengths, len);
-    ask<S, V>(Lane<T, Off>(p.dy, at, at.c), t0, last, d);
-    ask<S, VG>(Lane<G, Off>(p.gate, at, gate), t0, last, g);
-    ask<S, V>(Lane<T, Off>(p.y, at, at.c), t0 - 1, last, before);
+    ask<S, V, STREAM>(Lane<T, Off>(p.dy, at, at.c), t0, last, d);
+    ask<S, VG, STREAM && VG == V>(Lane<G, Off>(p.gate, at, gate), t0, last, g);
+    ask<S, V, STREAM>(Lane<T, Off>(p.y, at, at.c), t0 - 1, last, before);
   }
   float a[S][VG];
   take<S, V>(d, t0, len, all);
@@ -407,12 +408,12 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void scan_rows_bwd(tfft_scan_gra
       }
       const bool in = whole.value || t < f.length;
       const int own = whole.value ? V : at.own;
-      if (in) put<V>(dx.here(), r, own);
+      if (in) put<V, STREAM>(dx.here(), r, own);
       if (!kShared || (V == 1 && f.share == 1)) {
         Run<G, V> q;
 #pragma unroll
         for (int v = 0; v < V; ++v) q.set(v, da[v]);
-        if (in) put<V>(dg.here(), q, own);
+        if (in) put<V, STREAM>(dg.here(), q, own);
       } else if (lanes > 0) {
         sums[s] = da[0];
 #pragma unroll
@@ -526,22 +527,39 @@ static int lanes_of(const tfft_scan_grad_args& p) {
 }
 bool rows_sums_shares(const tfft_scan_grad_args& p) { return p.share > 1 && lanes_of(p) == 0; }
 
+// Rows that pass through in whole lines (the gate's too, where every channel has one): B = 8, L = 4096, D = 2048 with fp32 gates
+// takes 107 us forward and 174 back as a stream, 112 and 185 without; D = 2050, where tiles share lines, 140 and 263 against 120
+// and 219.
+static bool streams(std::initializer_list<std::pair<const tfft_seq_view*, int>> views, long long batch, long long length) {
+  for (const auto& [v, dtype] : views) {
+    const long long stride[2] = {v->batch, v->time}, extent[2] = {batch, length};
+    if (!whole_lines(v->data, dtype, stride, extent)) return false;
+  }
+  return true;
+}
+
 void launch_rows(const tfft_scan_args& p, const Chunking& c, word* words, hipStream_t s) {
   const bool vector = rows_vector(p);
+  const bool stream = p.channels % kRun == 0 && streams({{&p.x, p.dtype}, {&p.y, p.dtype}}, p.batch, p.length) &&
+                      (p.share > 1 || streams({{&p.gate, p.gate_dtype}}, p.batch, p.length));
   const Shape f = shape_of(p, c, run_of_call(p), through_batch(p), words);
   const dim3 grid((unsigned)c.blocks()), block(64 * c.waves);
   with_types(p.dtype, p.gate_dtype, [&](auto t, auto g) {
     using T = decltype(t);
     using G = decltype(g);
     constexpr int V = kRun;
-    if (!vector) scan_rows_fwd<T, G, 1, 1><<<grid, block, 0, s>>>(p, f);
-    else if (p.share == 1) scan_rows_fwd<T, G, V, V><<<grid, block, 0, s>>>(p, f);
-    else scan_rows_fwd<T, G, V, 1><<<grid, block, 0, s>>>(p, f);
+    if (!vector) scan_rows_fwd<T, G, 1, 1, false><<<grid, block, 0, s>>>(p, f);
+    else if (p.share == 1 && stream) scan_rows_fwd<T, G, V, V, true><<<grid, block, 0, s>>>(p, f);
+    else if (p.share == 1) scan_rows_fwd<T, G, V, V, false><<<grid, block, 0, s>>>(p, f);
+    else if (stream) scan_rows_fwd<T, G, V, 1, true><<<grid, block, 0, s>>>(p, f);
+    else scan_rows_fwd<T, G, V, 1, false><<<grid, block, 0, s>>>(p, f);
   });
 }
 
 void launch_rows(const tfft_scan_grad_args& p, const Chunking& c, word* words, float* parts, hipStream_t s) {
   const bool vector = rows_vector(p);
+  const bool stream = p.channels % kRun == 0 && streams({{&p.dy, p.dtype}, {&p.y, p.dtype}, {&p.dx, p.dtype}}, p.batch, p.length) &&
+                      (p.share > 1 || streams({{&p.gate, p.gate_dtype}, {&p.dgate, p.gate_dtype}}, p.batch, p.length));
   const Shape f = shape_of(p, c, run_of_call(p), through_batch(p), words);
   const dim3 grid((unsigned)c.blocks()), block(64 * c.waves);
   const int lanes = lanes_of(p);
@@ -549,9 +567,11 @@ void launch_rows(const tfft_scan_grad_args& p, const Chunking& c, word* words, f
     using T = decltype(t);
     using G = decltype(g);
     constexpr int V = kRun;
-    if (!vector) scan_rows_bwd<T, G, 1, 1><<<grid, block, 0, s>>>(p, f, parts, lanes);
-    else if (p.share == 1) scan_rows_bwd<T, G, V, V><<<grid, block, 0, s>>>(p, f, parts, lanes);
-    else scan_rows_bwd<T, G, V, 1><<<grid, block, 0, s>>>(p, f, parts, lanes);
+    if (!vector) scan_rows_bwd<T, G, 1, 1, false><<<grid, block, 0, s>>>(p, f, parts, lanes);
+    else if (p.share == 1 && stream) scan_rows_bwd<T, G, V, V, true><<<grid, block, 0, s>>>(p, f, parts, lanes);
+    else if (p.share == 1) scan_rows_bwd<T, G, V, V, false><<<grid, block, 0, s>>>(p, f, parts, lanes);
+    else if (stream) scan_rows_bwd<T, G, V, 1, true><<<grid, block, 0, s>>>(p, f, parts, lanes);
+    else scan_rows_bwd<T, G, V, 1, false><<<grid, block, 0, s>>>(p, f, parts, lanes);
     if (rows_sums_shares(p) && p.length > 0) {
       const long long n = p.batch * p.length * (p.channels / p.share);
       sum_shares<G><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(p, parts);

@@ -7,8 +7,11 @@ namespace {
 
 // A thread holds E consecutive steps of one row (batch entry, channel). Rows of up to 64 E steps: the next power of two
 // of lanes, several rows a wave. Longer rows: one a workgroup, in chunks of up to kMaxWaves waves.
-constexpr int kMaxWaves = 8, kMaxGroup = 64;
-constexpr int kSteps = 16;
+constexpr int kMaxGroup = 64;
+template <class T>
+constexpr int kSteps = 32 / sizeof(T);
+template <class T>
+constexpr int kMaxWaves = 4 * sizeof(T);  // chunks of 8192 steps
 
 struct Shape {
   long long rows;
@@ -97,7 +100,7 @@ __device__ __forceinline__ void scan_lanes(int lane, int width, float& A, float&
 }
 
 struct Lds {
-  float A[kMaxWaves], B[kMaxWaves], h;
+  float A[16], B[16], h;
   unsigned ticket;
 };
 
@@ -157,8 +160,8 @@ __device__ __forceinline__ bool take(const Shape& f, Lds& lds, long long* row, u
 }
 
 template <class T, class G>
-__global__ __launch_bounds__(64 * kMaxWaves) void scan_signals_fwd(tfft_scan_args p, Shape f) {
-  constexpr int E = kSteps;
+__global__ __launch_bounds__(64 * kMaxWaves<T>) void scan_signals_fwd(tfft_scan_args p, Shape f) {
+  constexpr int E = kSteps<T>;
   __shared__ Lds lds;
   long long row;
   unsigned chunk;
@@ -201,8 +204,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) void scan_signals_fwd(tfft_scan_arg
 
 // Backwards in time: the first thread has the latest steps, chunk 0 is the latest
 template <class T, class G>
-__global__ __launch_bounds__(64 * kMaxWaves) void scan_signals_bwd(tfft_scan_grad_args p, Shape f) {
-  constexpr int E = kSteps;
+__global__ __launch_bounds__(64 * kMaxWaves<T>) void scan_signals_bwd(tfft_scan_grad_args p, Shape f) {
+  constexpr int E = kSteps<T>;
   __shared__ Lds lds;
   long long row;
   unsigned chunk;
@@ -258,9 +261,10 @@ __global__ __launch_bounds__(64 * kMaxWaves) void scan_signals_bwd(tfft_scan_gra
   if (p.dinitial && live && chunk + 1 == (unsigned)f.chunks && piece == pieces - 1) p.dinitial[row] = k;
 }
 
-Chunking plan(long long batch, long long length, long long channels) {
+Chunking plan(long long batch, long long length, long long channels, int dtype) {
+  const int steps = dtype == TFFT_F32 ? kSteps<float> : kSteps<f16>, most = dtype == TFFT_F32 ? kMaxWaves<float> : kMaxWaves<f16>;
   Chunking c;
-  const long long rows = batch * channels, pieces = (length + kSteps - 1) / kSteps;
+  const long long rows = batch * channels, pieces = (length + steps - 1) / steps;
   c.tiles = rows;
   c.state_words = rows;
   c.group = kMaxGroup;
@@ -271,7 +275,7 @@ Chunking plan(long long batch, long long length, long long channels) {
     c.chunks = 1;
     return c;
   }
-  c.waves = (int)(pieces > 64 * (kMaxWaves - 1) ? kMaxWaves : (pieces + 63) / 64);
+  c.waves = (int)(pieces > 64 * (most - 1) ? most : (pieces + 63) / 64);
   c.chunks = (pieces + 64 * c.waves - 1) / (64 * c.waves);
   return c;
 }
@@ -295,8 +299,8 @@ bool signals_fit(const tfft_scan_args& p) {
 bool signals_fit(const tfft_scan_grad_args& p) {
   return p.share == 1 && p.dy.time == 1 && p.y.time == 1 && p.dx.time == 1 && p.dgate.time == 1 && p.gate.time <= 1;
 }
-Chunking plan_signals(const tfft_scan_args& p) { return plan(p.batch, p.length, p.channels); }
-Chunking plan_signals(const tfft_scan_grad_args& p) { return plan(p.batch, p.length, p.channels); }
+Chunking plan_signals(const tfft_scan_args& p) { return plan(p.batch, p.length, p.channels, p.dtype); }
+Chunking plan_signals(const tfft_scan_grad_args& p) { return plan(p.batch, p.length, p.channels, p.dtype); }
 
 void launch_signals(const tfft_scan_args& p, const Chunking& c, word* words, hipStream_t s) {
   const Shape f = shape_of(p, c, words);

@@ -1,5 +1,7 @@
 // Rotary positions: pairs of values times exp(2 pi i p F[i]) for 64-bit positions p and fixed-point frequencies F
 // (tfft_rotary). No counterpart in the reference.
+#include <type_traits>
+
 #include "seq_common.hpp"
 
 namespace {
@@ -53,7 +55,13 @@ struct Token {
         in_head(v.in_head), out_head(v.out_head) {}
 };
 
-template <class T, bool HALF, int NH>
+template <int R, bool STREAM, class T>
+__device__ __forceinline__ void put(T* to, const Run<T, R>& r, int valid) {
+  if constexpr (STREAM) store_run<T, R, true>(to, r);  // all units are whole
+  else store_some<R>(to, r, valid);
+}
+
+template <class T, bool HALF, int NH, bool STREAM>
 __global__ __launch_bounds__(256) void rotary_units(tfft_rotary_args p, Grid g) {
   constexpr int R = kRun<T>, pairs = HALF ? R : R / 2;
   const unsigned long long n = (unsigned long long)blockIdx.x * 256 + threadIdx.x;
@@ -119,9 +127,9 @@ __global__ __launch_bounds__(256) void rotary_units(tfft_rotary_args p, Grid g) 
           else re.set(2 * k, a), re.set(2 * k + 1, d);
         }
         x[j] = re;
-        if (HALF) store_some<R>(to[j] + half, im, valid);
+        if (HALF) put<R, STREAM>(to[j] + half, im, valid);
       }
-      store_some<R>(to[j], x[j], valid);
+      put<R, STREAM>(to[j], x[j], valid);
     }
   }
 }
@@ -151,13 +159,18 @@ extern "C" int tfft_rotary(const tfft_rotary_args* args, void* stream) {
   if (!p.tensor[1].in) p.tensor[1].heads = 0;
   if (p.batch > kMost || p.length > kMost || p.tensor[0].heads > kMost || p.tensor[1].heads > kMost)
     return refuse("an extent is too large");
-  bool in_place = true;
+  // Results that leave in whole lines and whole units are streamed: 8 x 4096 tokens with 32 + 8 heads of 128 in bf16 119 us
+  // against 126, 9003 tokens with 12 heads of 96 in fp32 15 against 17.
+  const int size = p.dtype == TFFT_F32 ? 4 : 2;
+  bool in_place = true, stream_out = p.rotary / 2 * size % 16 == 0 && p.head * size % 16 == 0;
   for (const tfft_rotary_view& v : p.tensor) {
     const long long extent[4] = {p.batch, p.length, v.heads, p.head};
     const long long in[4] = {v.in_batch, v.in_time, v.in_head, 1}, out[4] = {v.out_batch, v.out_time, v.out_head, 1};
     if (const char* why = check_tensor(v.in, p.dtype, in, extent, false)) return refuse(why);
     if (const char* why = check_tensor(v.out, p.dtype, out, extent, true)) return refuse(why);
     in_place = in_place && (v.heads == 0 || v.in == v.out);
+    const long long steps[3] = {v.out_batch, v.out_time, v.out_head}, counts[3] = {p.batch, p.length, v.heads};
+    stream_out = stream_out && (v.heads == 0 || whole_lines(v.out, p.dtype, steps, counts));
   }
   const int run = p.dtype == TFFT_F32 ? kRun<float> : kRun<f16>;
   Grid g;
@@ -175,13 +188,13 @@ extern "C" int tfft_rotary(const tfft_rotary_args* args, void* stream) {
   hipStream_t stream_ = static_cast<hipStream_t>(stream);
   const auto launch = [&](auto t) {
     using T = decltype(t);
-    if (p.pairs == TFFT_PAIRS_HALF) {
-      if (many) rotary_units<T, true, kHeads><<<grid, 256, 0, stream_>>>(p, g);
-      else rotary_units<T, true, 1><<<grid, 256, 0, stream_>>>(p, g);
-    } else {
-      if (many) rotary_units<T, false, kHeads><<<grid, 256, 0, stream_>>>(p, g);
-      else rotary_units<T, false, 1><<<grid, 256, 0, stream_>>>(p, g);
-    }
+    const auto pairs = [&](auto half) {
+      if (!many) rotary_units<T, half.value, 1, false><<<grid, 256, 0, stream_>>>(p, g);
+      else if (stream_out) rotary_units<T, half.value, kHeads, true><<<grid, 256, 0, stream_>>>(p, g);
+      else rotary_units<T, half.value, kHeads, false><<<grid, 256, 0, stream_>>>(p, g);
+    };
+    if (p.pairs == TFFT_PAIRS_HALF) pairs(std::true_type());
+    else pairs(std::false_type());
   };
   if (p.dtype == TFFT_F32) launch(float());
   else if (p.dtype == TFFT_F16) launch(f16());
