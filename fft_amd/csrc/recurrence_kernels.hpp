@@ -33,15 +33,17 @@ struct Chunking {
   int waves = 0;         // of a workgroup
   int group = 1;         // chunks whose (A, B) are joined directly; the state behind each group is handed on
   int lanes = 64;        // signals: threads of a row, where a wave holds several rows
+  bool walks = false;    // a workgroup takes all chunks of its tile, one after the other
   long long state_words = 0;  // states of one chunk
   // 64-bit words: the counters, a map a state and chunk where groups are used, half a word a state and group
   long long words() const {
-    return chunks <= 1 ? 0 : kCounterWords * counters() + state_words * (group > 1 ? chunks : 0) +
+    return apart() <= 1 ? 0 : kCounterWords * counters() + state_words * (group > 1 ? chunks : 0) +
                                  (state_words * ((chunks + group - 1) / group) + 1) / 2;
   }
+  long long apart() const { return walks ? 1 : chunks; }  // chunks that workgroups of their own take
   int counters() const { return tiles >= kManyTiles ? 8 : 1; }
   // workgroups; a few find no ticket left where the tiles do not divide evenly
-  long long blocks() const { return chunks <= 1 ? tiles : (tiles + counters() - 1) / counters() * counters() * chunks; }
+  long long blocks() const { return apart() <= 1 ? tiles : (tiles + counters() - 1) / counters() * counters() * chunks; }
 };
 
 // Tile and chunk of this workgroup, the same for all threads; false where there is none left. `shared` lies in LDS.
@@ -49,7 +51,7 @@ struct Turns {
   unsigned tiles, counters, chunks;
 };
 inline Turns turns_of(const Chunking& c) {
-  return Turns{(unsigned)c.tiles, (unsigned)c.counters(), (unsigned)c.chunks};
+  return Turns{(unsigned)c.tiles, (unsigned)c.counters(), (unsigned)c.apart()};
 }
 __device__ __forceinline__ bool take_turn(const Turns& f, word* words, unsigned* shared, unsigned* tile, unsigned* chunk) {
   if (f.chunks <= 1) {

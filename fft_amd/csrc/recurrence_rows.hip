@@ -473,9 +473,11 @@ Chunking plan(long long batch, long long length, long long channels, int run, bo
   Chunking c;
   const long long padded = (channels + run - 1) / run * run, width = 64 * run;
   c.tiles = through ? (batch * padded + width - 1) / width : batch * ((channels + width - 1) / width);
-  c.waves = (int)(length > (kMaxWaves - 1) * steps ? kMaxWaves : length < steps ? 1 : (length + steps - 1) / steps);
-  c.chunks = (length + c.waves * steps - 1) / (c.waves * steps);
-  if (c.chunks < 1) c.chunks = 1;
+  // as few chunks as the workgroup's waves allow, then as few waves as those need
+  const long long pieces = length > 0 ? (length + steps - 1) / steps : 1;
+  c.chunks = (pieces + kMaxWaves - 1) / kMaxWaves;
+  c.waves = (int)((pieces + c.chunks - 1) / c.chunks);
+  c.chunks = (pieces + c.waves - 1) / c.waves;
   c.state_words = c.tiles * width;
   // About kResident workgroups run at once, kResident / tiles chunks of each tile. That many are joined directly, so that few
   // channels wait for one state in that many chunks, and many channels do not read what they need not: B = 8,

@@ -8,6 +8,12 @@ namespace {
 // A thread holds E consecutive steps of one row (batch entry, channel). Rows of up to 64 E steps: the next power of two
 // of lanes, several rows a wave. Longer rows: one a workgroup, in chunks of up to kMaxWaves waves.
 constexpr int kMaxGroup = 64;
+// Longer rows that are many are walked by a workgroup each, chunk after chunk, few rows are split: 256 x 20000 in bf16 takes 11 us
+// walked against 13 split, 256 x 100000 in fp32 65 against 69, 16 x 2^20 47 split (16 workgroups would walk). From kShortChunks
+// rows on the workgroups have 4 waves, and several of a CU load, wait and store at different times: 49152 x 8200 in bf16 449 us
+// forward and 769 back against 657 and 1351 with 8 waves; with 256 rows they are too few, 96 and 125 us against 65 and 110.
+constexpr int kManyRows = 256, kShortChunks = 1024, kWalkWaves = 4;
+enum { ONE, WALK, SPLIT };  // one chunk, or chunks after one another, or apart
 template <class T>
 constexpr int kSteps = 32 / sizeof(T);
 template <class T>
@@ -53,9 +59,43 @@ __device__ __forceinline__ void line_up(Run<T, E>& r, int t0, int length) {
     for (int i = 0; i < kWords; ++i) r.w[i] = by & 1 ? r.w[i] >> 16 | (i + 1 < kWords ? r.w[i + 1] << 16 : 0u) : r.w[i];
   }
 }
-template <int E, class T>
+// The first `valid` of E elements, fewer than E: halves, quarters and so on as the bits of `valid` say, what follows moved down
+template <int N, class T, int E>
+__device__ __forceinline__ void store_head(T* p, Run<T, E> r, int valid) {
+  if constexpr (N > 1) {
+    constexpr int kWords = N / 2 * sizeof(T) / 4;  // of the half; 0: half a word
+    if (valid & (N / 2)) {
+      if constexpr (kWords == 0) {
+        Run<T, 1> one;
+        one.w[0] = r.w[0];
+        store_run<T, 1>(p, one);
+      } else {
+        __builtin_memcpy(p, r.w, 4 * kWords);
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) r.w[i] = r.w[i + kWords];
+      }
+      p += N / 2;
+    }
+    store_head<N / 2>(p, r, valid);
+  }
+}
+// STREAM: as in load_run. Two stores share a line here, which costs a row in one workgroup 1 to 8 %, but where chunks are taken apart the
+// states come through faster: two entries of 8 signals of 1048573 steps in fp32 take 47 us forward and 74 back against 53 and 90.
+template <int E, bool STREAM, class T>
 __device__ __forceinline__ void store_steps(T* p, int t0, int length, const Run<T, E>& r) {
-  store_some<E>(p + t0, r, min(max(length - t0, 0), E));
+  const int valid = min(max(length - t0, 0), E);
+  if (STREAM && valid == E) {
+    using Words = uint32_t __attribute__((ext_vector_type(4), aligned(2)));
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(r.w) / 4; i += 4) {
+      const Words w = {r.w[i], r.w[i + 1], r.w[i + 2], r.w[i + 3]};
+      __builtin_nontemporal_store(w, (Words*)(p + t0) + i / 4);
+    }
+  } else if (valid == E) {
+    store_run<T, E>(p + t0, r);
+  } else {
+    store_head<E>(p + t0, r, valid);
+  }
 }
 
 // Decays of E steps that were asked for; 1 behind the sequence. time is 1, or 0 for one decay throughout.
@@ -104,13 +144,14 @@ struct Lds {
   unsigned ticket;
 };
 
-// The state in front of this thread's piece from its (A, B) and `h`, the state before the first chunk. `order`: 0 for the
-// thread that comes first.
+// The state in front of this thread's piece from its (A, B) and `h`, the state in front of the chunk, or where chunks are taken
+// apart of the first one. `order`: 0 for the thread that comes first.
+template <int MODE>
 __device__ __forceinline__ float state_in_front(const Shape& f, Lds& lds, unsigned chunk, long long row, int order, float A, float B, float h) {
   const int lane = order & 63, wave = order >> 6, waves = blockDim.x >> 6;
   float front_a, front_b;
   scan_lanes(lane, f.lanes, A, B, front_a, front_b);
-  if (f.lanes < 64 || (waves == 1 && f.chunks <= 1)) return join(front_a, h, front_b);
+  if (f.lanes < 64 || (MODE == ONE && waves == 1)) return join(front_a, h, front_b);
   if (lane == 63) lds.A[wave] = A, lds.B[wave] = B;
   __syncthreads();
   float wave_a = 1.0f, wave_b = 0.0f;
@@ -118,7 +159,7 @@ __device__ __forceinline__ float state_in_front(const Shape& f, Lds& lds, unsign
     wave_b = join(lds.A[w], wave_b, lds.B[w]);
     wave_a *= lds.A[w];
   }
-  if (f.chunks > 1) {
+  if constexpr (MODE == SPLIT) {
     if (wave == waves - 1) {
       const int r = chunk % f.group, q = chunk / f.group;
       const bool more = chunk + 1 < (unsigned)f.chunks;
@@ -147,116 +188,137 @@ __device__ __forceinline__ float state_in_front(const Shape& f, Lds& lds, unsign
   return join(front_a, h, front_b);
 }
 
-// Row and chunk of this thread
+// Row of this thread, and its chunk where chunks are taken apart
+template <int MODE>
 __device__ __forceinline__ bool take(const Shape& f, Lds& lds, long long* row, unsigned* chunk) {
-  if (f.lanes < 64) {
-    *row = ((long long)blockIdx.x * blockDim.x + threadIdx.x) / f.lanes, *chunk = 0;
+  *chunk = 0;
+  if constexpr (MODE == SPLIT) {
+    unsigned tile;
+    const bool there = take_turn(f.turns, f.words, &lds.ticket, &tile, chunk);
+    *row = tile;
+    return there;
+  } else {
+    *row = f.lanes < 64 ? ((long long)blockIdx.x * blockDim.x + threadIdx.x) / f.lanes : (long long)blockIdx.x;
     return true;
   }
-  unsigned tile;
-  const bool there = take_turn(f.turns, f.words, &lds.ticket, &tile, chunk);
-  *row = tile;
-  return there;
 }
 
-template <class T, class G>
+// The state behind the chunk, for all threads of a workgroup that walks on; it is the one of the thread that comes last
+__device__ __forceinline__ float state_behind(Lds& lds, bool mine, float h) {
+  if (mine) lds.h = h;
+  __syncthreads();
+  return lds.h;
+}
+
+template <class T, class G, int MODE>
 __global__ __launch_bounds__(64 * kMaxWaves<T>) void scan_signals_fwd(tfft_scan_args p, Shape f) {
   constexpr int E = kSteps<T>;
   __shared__ Lds lds;
   long long row;
   unsigned chunk;
-  if (!take(f, lds, &row, &chunk)) return;
+  if (!take<MODE>(f, lds, &row, &chunk)) return;
   const bool live = row < f.rows;
   if (!live) row = 0;
-  const int b = (int)(row / f.channels), c = (int)(row % f.channels);
+  const int b = (int)(row / f.channels), c = (int)(row % f.channels), len = live ? steps_of(p.lengths, b, f.length) : 0;
   const int order = threadIdx.x, piece = f.lanes < 64 ? order & (f.lanes - 1) : order;
-  const int t0 = (int)(chunk * blockDim.x + piece) * E, len = live ? steps_of(p.lengths, b, f.length) : 0;
+  const int pieces = f.lanes < 64 ? f.lanes : (int)blockDim.x;
   const T* x = (const T*)p.x.data + b * p.x.batch + c * p.x.channel;
   const G* g = (const G*)p.gate.data + b * p.gate.batch + c * p.gate.channel;
-  const float initial = p.initial ? p.initial[row] : 0.0f;
-  Run<T, E> xr;
-  Run<G, E> gr;
-  if (f.length > 0) {
-    xr = ask<E>(x, t0, f.length);
-    gr = p.gate.time ? ask<E>(g, t0, f.length) : one<E>(g);
-  }
-  take<E>(xr, t0, len, f.length);
-  float a[E];
-  take_decays<E>(gr, p.gate.time, t0, len, f.length, f.log_gate, a);
-  float h = initial;
-  float A = 1.0f, B = 0.0f;
+  T* y = (T*)p.y.data + b * p.y.batch + c * p.y.channel;
+  float start = p.initial ? p.initial[row] : 0.0f, h;
+  while (true) {
+    const int t0 = (int)(chunk * pieces + piece) * E;
+    Run<T, E> xr;
+    Run<G, E> gr;
+    if (f.length > 0) {
+      xr = ask<E>(x, t0, f.length);
+      gr = p.gate.time ? ask<E>(g, t0, f.length) : one<E>(g);
+    }
+    take<E>(xr, t0, len, f.length);
+    float a[E];
+    take_decays<E>(gr, p.gate.time, t0, len, f.length, f.log_gate, a);
+    float A = 1.0f, B = 0.0f;
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
-    A *= a[i];
-    B = fmaf(a[i], B, xr.get(i));
-  }
-  h = state_in_front(f, lds, chunk, row, order, A, B, h);
-  Run<T, E> r;
+    for (int i = 0; i < E; ++i) {
+      A *= a[i];
+      B = fmaf(a[i], B, xr.get(i));
+    }
+    h = state_in_front<MODE>(f, lds, chunk, row, order, A, B, start);
+    Run<T, E> r;
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
-    h = fmaf(a[i], h, xr.get(i));
-    r.set(i, t0 + i < len ? h : 0.0f);
+    for (int i = 0; i < E; ++i) {
+      h = fmaf(a[i], h, xr.get(i));
+      r.set(i, t0 + i < len ? h : 0.0f);
+    }
+    if (live) store_steps<E, MODE == SPLIT>(y, t0, f.length, r);
+    if (MODE != WALK || chunk + 1 == (unsigned)f.chunks) break;
+    start = state_behind(lds, piece == pieces - 1, h);
+    ++chunk;
   }
-  if (live) store_steps<E>((T*)p.y.data + b * p.y.batch + c * p.y.channel, t0, f.length, r);
-  const int pieces = f.lanes < 64 ? f.lanes : (int)blockDim.x;
   if (p.last && live && chunk + 1 == (unsigned)f.chunks && piece == pieces - 1) p.last[row] = h;
 }
 
 // Backwards in time: the first thread has the latest steps, chunk 0 is the latest
-template <class T, class G>
+template <class T, class G, int MODE>
 __global__ __launch_bounds__(64 * kMaxWaves<T>) void scan_signals_bwd(tfft_scan_grad_args p, Shape f) {
   constexpr int E = kSteps<T>;
   __shared__ Lds lds;
   long long row;
   unsigned chunk;
-  if (!take(f, lds, &row, &chunk)) return;
+  if (!take<MODE>(f, lds, &row, &chunk)) return;
   const bool live = row < f.rows;
   if (!live) row = 0;
-  const int b = (int)(row / f.channels), c = (int)(row % f.channels);
+  const int b = (int)(row / f.channels), c = (int)(row % f.channels), len = live ? steps_of(p.lengths, b, f.length) : 0;
   const int order = threadIdx.x, piece = f.lanes < 64 ? order & (f.lanes - 1) : order;
   const int pieces = f.lanes < 64 ? f.lanes : (int)blockDim.x;
-  const int t0 = ((int)(f.chunks - 1 - chunk) * pieces + pieces - 1 - piece) * E, len = live ? steps_of(p.lengths, b, f.length) : 0;
   const T* dy = (const T*)p.dy.data + b * p.dy.batch + c * p.dy.channel;
   const T* y = (const T*)p.y.data + b * p.y.batch + c * p.y.channel;
   const G* g = (const G*)p.gate.data + b * p.gate.batch + c * p.gate.channel;
-  const float start = p.initial ? p.initial[row] : 0.0f, dlast = p.dlast ? p.dlast[row] : 0.0f;
-  Run<T, E> d, own;
-  Run<T, 1> before;
-  Run<G, E> gr;
-  if (f.length > 0) {
-    d = ask<E>(dy, t0, f.length);
-    gr = p.gate.time ? ask<E>(g, t0, f.length) : one<E>(g);
-    own = ask<E>(y, t0, f.length);
-    before = load_run<T, 1>(y + min(max(t0 - 1, 0), f.length - 1));
-  }
-  take<E>(d, t0, len, f.length);
-  float a[E];
-  take_decays<E>(gr, p.gate.time, t0, len, f.length, f.log_gate, a);
-  float A = 1.0f, B = 0.0f;
+  const float initial = p.initial ? p.initial[row] : 0.0f;
+  float start = p.dlast ? p.dlast[row] : 0.0f, k;
+  while (true) {
+    const int t0 = ((int)(f.chunks - 1 - chunk) * pieces + pieces - 1 - piece) * E;
+    Run<T, E> d, own;
+    Run<T, 1> before;
+    Run<G, E> gr;
+    if (f.length > 0) {
+      d = ask<E>(dy, t0, f.length);
+      gr = p.gate.time ? ask<E>(g, t0, f.length) : one<E>(g);
+      own = ask<E>(y, t0, f.length);
+      before = load_run<T, 1>(y + min(max(t0 - 1, 0), f.length - 1));
+    }
+    take<E>(d, t0, len, f.length);
+    float a[E];
+    take_decays<E>(gr, p.gate.time, t0, len, f.length, f.log_gate, a);
+    float A = 1.0f, B = 0.0f;
 #pragma unroll
-  for (int i = E - 1; i >= 0; --i) {
-    A *= a[i];
-    B = a[i] * (B + d.get(i));
-  }
-  float k = state_in_front(f, lds, chunk, row, order, A, B, dlast);
-  take<E>(own, t0, len, f.length);
-  float dx[E], dgate[E];
+    for (int i = E - 1; i >= 0; --i) {
+      A *= a[i];
+      B = a[i] * (B + d.get(i));
+    }
+    k = state_in_front<MODE>(f, lds, chunk, row, order, A, B, start);
+    take<E>(own, t0, len, f.length);
+    float dx[E], dgate[E];
 #pragma unroll
-  for (int i = E - 1; i >= 0; --i) {
-    const float e = d.get(i) + k;
-    const float state = i > 0 ? own.get(i > 0 ? i - 1 : 0) : t0 > 0 ? before.get(0) : start;
-    const bool inside = t0 + i < len;
-    dgate[i] = inside ? e * state * (f.log_gate ? a[i] : 1.0f) : 0.0f;
-    dx[i] = inside ? e : 0.0f;
-    k = a[i] * e;
-  }
-  Run<T, E> r;
-  Run<G, E> q;
+    for (int i = E - 1; i >= 0; --i) {
+      const float e = d.get(i) + k;
+      const float state = i > 0 ? own.get(i > 0 ? i - 1 : 0) : t0 > 0 ? before.get(0) : initial;
+      const bool inside = t0 + i < len;
+      dgate[i] = inside ? e * state * (f.log_gate ? a[i] : 1.0f) : 0.0f;
+      dx[i] = inside ? e : 0.0f;
+      k = a[i] * e;
+    }
+    Run<T, E> r;
+    Run<G, E> q;
 #pragma unroll
-  for (int i = 0; i < E; ++i) r.set(i, dx[i]), q.set(i, dgate[i]);
-  if (live) {
-    store_steps<E>((T*)p.dx.data + b * p.dx.batch + c * p.dx.channel, t0, f.length, r);
-    store_steps<E>((G*)p.dgate.data + b * p.dgate.batch + c * p.dgate.channel, t0, f.length, q);
+    for (int i = 0; i < E; ++i) r.set(i, dx[i]), q.set(i, dgate[i]);
+    if (live) {
+      store_steps<E, MODE == SPLIT>((T*)p.dx.data + b * p.dx.batch + c * p.dx.channel, t0, f.length, r);
+      store_steps<E, MODE == SPLIT && sizeof(G) == sizeof(T)>((G*)p.dgate.data + b * p.dgate.batch + c * p.dgate.channel, t0, f.length, q);
+    }
+    if (MODE != WALK || chunk + 1 == (unsigned)f.chunks) break;
+    start = state_behind(lds, piece == pieces - 1, k);
+    ++chunk;
   }
   if (p.dinitial && live && chunk + 1 == (unsigned)f.chunks && piece == pieces - 1) p.dinitial[row] = k;
 }
@@ -275,7 +337,10 @@ Chunking plan(long long batch, long long length, long long channels, int dtype) 
     c.chunks = 1;
     return c;
   }
-  c.waves = (int)(pieces > 64 * (most - 1) ? most : (pieces + 63) / 64);
+  c.walks = pieces > 64 * most && rows >= kManyRows;
+  const int waves = c.walks && rows >= kShortChunks ? kWalkWaves : most;
+  c.chunks = (pieces + 64 * waves - 1) / (64 * waves);
+  c.waves = (int)((pieces + 64 * c.chunks - 1) / (64 * c.chunks));
   c.chunks = (pieces + 64 * c.waves - 1) / (64 * c.waves);
   return c;
 }
@@ -305,13 +370,21 @@ Chunking plan_signals(const tfft_scan_grad_args& p) { return plan(p.batch, p.len
 void launch_signals(const tfft_scan_args& p, const Chunking& c, word* words, hipStream_t s) {
   const Shape f = shape_of(p, c, words);
   with_types(p.dtype, p.gate_dtype, [&](auto t, auto g) {
-    scan_signals_fwd<decltype(t), decltype(g)><<<grid_of(c), dim3(64 * c.waves), 0, s>>>(p, f);
+    using T = decltype(t);
+    using G = decltype(g);
+    if (c.chunks <= 1) scan_signals_fwd<T, G, ONE><<<grid_of(c), dim3(64 * c.waves), 0, s>>>(p, f);
+    else if (c.walks) scan_signals_fwd<T, G, WALK><<<grid_of(c), dim3(64 * c.waves), 0, s>>>(p, f);
+    else scan_signals_fwd<T, G, SPLIT><<<grid_of(c), dim3(64 * c.waves), 0, s>>>(p, f);
   });
 }
 void launch_signals(const tfft_scan_grad_args& p, const Chunking& c, word* words, hipStream_t s) {
   const Shape f = shape_of(p, c, words);
   with_types(p.dtype, p.gate_dtype, [&](auto t, auto g) {
-    scan_signals_bwd<decltype(t), decltype(g)><<<grid_of(c), dim3(64 * c.waves), 0, s>>>(p, f);
+    using T = decltype(t);
+    using G = decltype(g);
+    if (c.chunks <= 1) scan_signals_bwd<T, G, ONE><<<grid_of(c), dim3(64 * c.waves), 0, s>>>(p, f);
+    else if (c.walks) scan_signals_bwd<T, G, WALK><<<grid_of(c), dim3(64 * c.waves), 0, s>>>(p, f);
+    else scan_signals_bwd<T, G, SPLIT><<<grid_of(c), dim3(64 * c.waves), 0, s>>>(p, f);
   });
 }
 
