@@ -84,15 +84,14 @@ __device__ __forceinline__ void store_head(T* p, Run<T, E> r, int valid) {
 template <int E, bool STREAM, class T>
 __device__ __forceinline__ void store_steps(T* p, int t0, int length, const Run<T, E>& r) {
   const int valid = min(max(length - t0, 0), E);
-  if (STREAM && valid == E) {
-    using Words = uint32_t __attribute__((ext_vector_type(4), aligned(2)));
+  if (valid == E) {
+    using Words = uint32_t __attribute__((ext_vector_type(4), aligned(2)));  // 16 bytes, or the compiler cuts them up otherwise
 #pragma unroll
     for (int i = 0; i < (int)sizeof(r.w) / 4; i += 4) {
       const Words w = {r.w[i], r.w[i + 1], r.w[i + 2], r.w[i + 3]};
-      __builtin_nontemporal_store(w, (Words*)(p + t0) + i / 4);
+      if (STREAM) __builtin_nontemporal_store(w, (Words*)(p + t0) + i / 4);
+      else ((Words*)(p + t0))[i / 4] = w;
     }
-  } else if (valid == E) {
-    store_run<T, E>(p + t0, r);
   } else {
     store_head<E>(p + t0, r, valid);
   }
