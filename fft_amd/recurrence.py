@@ -26,9 +26,10 @@ def _refuse(message, code=3):
 
 def _placed(call, device, stream, *args):
     """call(*args, raw stream) with torch's current device and stream those of the call, so that what it allocates belongs to
-    the stream that it runs on. Switching costs more than a short kernel, so it is left out where nothing changes."""
-    if stream is None and device.index == torch.cuda.current_device():
-        return call(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    the stream that it runs on. device: an index. Switching costs more than a short kernel, so it is left out where nothing
+    changes."""
+    if stream is None and device == torch.cuda.current_device():
+        return call(*args, torch._C._cuda_getCurrentRawStream(device))
     with torch.cuda.device(device):
         if stream is None:
             return call(*args, torch.cuda.current_stream(device).cuda_stream)
@@ -46,12 +47,13 @@ def _types(who, x, gate):
 
 
 def _same_device(who, x, *others):
+    """Index of the device that all tensors lie on"""
     if not x.is_cuda:
         _refuse(f"{who} needs device tensors")
-    device = x.device
+    device = x.get_device()
     for t in others:
-        if t is not None and t.device != device:
-            _refuse(f"{who}: tensors on {device} and {t.device}")
+        if t is not None and t.get_device() != device:
+            _refuse(f"{who}: tensors on {x.device} and {t.device}")
     return device
 
 
@@ -91,7 +93,7 @@ def _sizes(who, x, gate, dim):
 
 def _out(who, name, t, like):
     if t is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+        return torch.empty_like(like, memory_format=torch.contiguous_format)
     if t.dtype != like.dtype or t.shape != like.shape:
         _refuse(f"{who}: {name} is a {like.dtype} tensor {tuple(like.shape)}")
     return t
@@ -178,14 +180,15 @@ def _gated_scan_step(x, gate, state, log_gate, new_state, out, stream):
     code, gate_code = _types(who, x, gate)
     if x.dim() != 2 or gate.dim() != 2 or gate.shape[0] != x.shape[0]:
         _refuse(f"{who} needs x [B, D] and gate [B, G], got {tuple(x.shape)} and {tuple(gate.shape)}")
-    B, D = x.shape
+    shape = x.shape
+    B, D = shape
     G = gate.shape[1]
     if D > 0 if G < 1 else D % G:
         _refuse(f"{who}: {G} gates do not divide {D} channels")
     if new_state is None:
         new_state = state
-    for t in (state, new_state):
-        if t.dtype != torch.float32 or t.shape != x.shape:
+    for t in (state,) if new_state is state else (state, new_state):
+        if t.dtype != torch.float32 or t.shape != shape:
             _refuse(f"{who}: state and new_state are float32 tensors [{B}, {D}]")
     y = _out(who, "out", out, x)
     rows = []

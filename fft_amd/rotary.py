@@ -15,9 +15,10 @@ import torch
 
 from . import _lib
 from .api import _check
-from .recurrence import _FLOATS, _placed, _refuse
+from .recurrence import _FLOATS, _placed, _refuse, _same_device
 
 _PAIRS = {"half": 0, "interleaved": 1}
+_POSITIONS = {torch.int64: 8, torch.int32: 4}
 
 
 class RotaryPlan:
@@ -78,9 +79,8 @@ def rotate(plan, q, k=None, positions=None, pairs="half", inverse=False, first=0
     2 i with 2 i + 1. positions: int64 or int32 [B, L] or [L] on the device (negative ones turn backwards); without
     them position t is first + t. inverse: the other way round, which is the gradient of rotate. out, out_k: tensors for the results,
     q and k themselves allowed. Asynchronous on `stream` (default: torch's current stream)."""
-    if not q.is_cuda:
-        _refuse("rotate needs device tensors")
-    return _placed(_rotate, q.device, stream, plan, q, k, positions, pairs, inverse, first, out, out_k)
+    device = _same_device("rotate", q, k, plan.turns, positions, out, out_k)
+    return _placed(_rotate, device, stream, plan, q, k, positions, pairs, inverse, first, out, out_k)
 
 
 _NO_TENSOR = (0,) * 9
@@ -88,52 +88,59 @@ _NO_TENSOR = (0,) * 9
 
 def _rotate(plan, q, k, positions, pairs, inverse, first, out, out_k, stream):
     who = "rotate"
-    code = _FLOATS.get(q.dtype)
+    dtype, shape = q.dtype, q.shape
+    code = _FLOATS.get(dtype)
     if code is None:
-        _refuse(f"{who}: unsupported element type {q.dtype}", 1)
+        _refuse(f"{who}: unsupported element type {dtype}", 1)
     if pairs not in _PAIRS:
         _refuse(f"{who}: pairs is 'half' or 'interleaved', not {pairs!r}")
-    if q.dim() != 4:
-        _refuse(f"{who}: q is [batch, time, heads, values], got {tuple(q.shape)}")
-    B, L, _, P = q.shape
+    if len(shape) != 4:
+        _refuse(f"{who}: q is [batch, time, heads, values], got {tuple(shape)}")
+    B, L, H, P = shape
     if plan.size > P:
         _refuse(f"{who}: the plan rotates {plan.size} values, a head has {P}")
-    if k is None and out_k is not None:
-        _refuse(f"{who}: out_k without k")
-    device = q.device
-    for t in (plan.turns, k, positions, out, out_k):
-        if t is not None and t.device != device:
-            _refuse(f"{who}: tensors on {device} and {t.device}")
-    position_bytes = position_batch = position_time = 0
+    at = position_bytes = position_batch = position_time = 0
     if positions is not None:
-        if positions.dtype not in (torch.int64, torch.int32):
+        position_bytes = _POSITIONS.get(positions.dtype)
+        if position_bytes is None:
             _refuse(f"{who}: positions are int64 or int32, not {positions.dtype}")
-        if positions.shape != (B, L) and positions.shape != (L,):
+        if positions.shape == (B, L):
+            position_batch, position_time = positions.stride()
+        elif positions.shape == (L,):
+            position_time = positions.stride(0)
+        else:
             _refuse(f"{who}: positions {tuple(positions.shape)} are neither [{B}, {L}] nor [{L}]")
-        position_bytes = positions.element_size()
-        position_batch = positions.stride(0) if positions.dim() == 2 else 0
-        position_time = positions.stride(-1)
-    views, results = [], []
-    for t, o in ((q, out), (k, out_k)):
-        if t is None:
-            views += _NO_TENSOR
-            continue
-        if t.dim() != 4 or t.dtype != q.dtype or t.shape[0] != B or t.shape[1] != L or t.shape[3] != P:
-            _refuse(f"{who}: k is a {q.dtype} tensor [{B}, {L}, heads, {P}]")
-        if o is None:
-            o = torch.empty(t.shape, dtype=t.dtype, device=device)
-        elif o.dtype != t.dtype or o.shape != t.shape:
-            _refuse(f"{who}: a result is a {t.dtype} tensor {tuple(t.shape)}")
-        *steps, one = t.stride()
-        *out_steps, out_one = o.stride()
-        if P > 1 and (one != 1 or out_one != 1):
-            _refuse(f"{who}: the values of a head are contiguous")
-        results.append(o)
-        views += (t.data_ptr(), o.data_ptr(), t.shape[2], *steps, *out_steps)
+        at = positions.data_ptr()
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.dtype != dtype or out.shape != shape:
+        _refuse(f"{who}: the result of q is a {dtype} tensor {tuple(shape)}")
+    first_view = _view(who, q, out, H, P)
+    if k is None:
+        if out_k is not None:
+            _refuse(f"{who}: out_k without k")
+        second_view = _NO_TENSOR
+    else:
+        k_shape = k.shape
+        if k.dtype != dtype or len(k_shape) != 4 or k_shape[0] != B or k_shape[1] != L or k_shape[3] != P:
+            _refuse(f"{who}: k is a {dtype} tensor [{B}, {L}, heads, {P}]")
+        if out_k is None:
+            out_k = torch.empty_like(k, memory_format=torch.contiguous_format)
+        elif out_k.dtype != dtype or out_k.shape != k_shape:
+            _refuse(f"{who}: the result of k is a {dtype} tensor {tuple(k_shape)}")
+        second_view = _view(who, k, out_k, k_shape[2], P)
     rc = _lib.load().tfft_rotary(
         _lib.ROTARY_ARGS.pack(_lib.ROTARY_ARGS.size, code, _PAIRS[pairs], bool(inverse), B, L, P, plan.size, plan.magnitude,
-                              position_bytes, plan.turns.data_ptr(), 0 if positions is None else positions.data_ptr(),
-                              position_batch, position_time, int(first), *views), stream)
+                              position_bytes, plan.turns.data_ptr(), at, position_batch, position_time, int(first),
+                              *first_view, *second_view), stream)
     if rc:
         _check(rc)
-    return results[0] if k is None else tuple(results)
+    return out if k is None else (out, out_k)
+
+
+def _view(who, t, out, heads, values):
+    a, b, c, one = t.stride()
+    d, e, f, out_one = out.stride()
+    if values > 1 and (one != 1 or out_one != 1):
+        _refuse(f"{who}: the values of a head are contiguous")
+    return t.data_ptr(), out.data_ptr(), heads, a, b, c, d, e, f
