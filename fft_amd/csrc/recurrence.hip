@@ -132,13 +132,31 @@ template <class P>
 unsigned long long workspace_of(const P& p) {
   return 8ull * plan_of(p).words() + parts_of(p);
 }
+// A launch counts its threads in 32 bits
 template <class P>
 const char* check_plan(const P& p) {
   const char* large = "more sequences or steps than one launch takes";
-  if (p.batch * (p.channels + 3) > kMaxExtent || (p.share > 1 && (__int128)p.batch * p.length * p.channels > ((__int128)1 << 38)))
-    return large;
+  constexpr long long most = 0xffff0000LL;
+  if (p.batch * (p.channels + 3) > kMaxExtent) return large;
   const Chunking c = plan_of(p);
-  return c.blocks() > kMaxExtent ? large : nullptr;
+  if ((__int128)c.blocks() * 64 * c.waves > most) return large;
+  return parts_of(p) && (__int128)p.batch * p.length * (p.channels / p.share) > most ? large : nullptr;
+}
+
+// Two tensors at one address: outputs take an input's place element for element, or none at all
+bool same(const void* a, const void* b) { return a && a == b; }
+bool alike(const tfft_seq_view& a, const tfft_seq_view& b) {
+  return a.batch == b.batch && a.time == b.time && a.channel == b.channel;
+}
+const char* check_places(const tfft_scan_args& p) {
+  if (same(p.y.data, p.gate.data)) return "y may not take the gate's place";
+  return same(p.y.data, p.x.data) && !alike(p.x, p.y) ? "in place needs equal strides on both sides" : nullptr;
+}
+const char* check_places(const tfft_scan_grad_args& p) {
+  for (const tfft_seq_view* v : {&p.dy, &p.y, &p.gate, &p.dx})
+    if (same(p.dgate.data, v->data)) return "dgate may not take another tensor's place";
+  if (same(p.dx.data, p.y.data) || same(p.dx.data, p.gate.data)) return "dx may not take y's or the gate's place";
+  return same(p.dx.data, p.dy.data) && !alike(p.dx, p.dy) ? "in place needs equal strides on both sides" : nullptr;
 }
 
 template <class P>
@@ -179,6 +197,7 @@ extern "C" int tfft_scan_forward(const tfft_scan_args* args, void* stream) {
   TFFT_SEQ_CHECK(check_view(p.x, p.dtype, p.batch, p.length, p.channels, false));
   TFFT_SEQ_CHECK(check_view(p.gate, p.gate_dtype, p.batch, p.length, p.channels / p.share, false));
   TFFT_SEQ_CHECK(check_view(p.y, p.dtype, p.batch, p.length, p.channels, true));
+  if (p.length > 0) TFFT_SEQ_CHECK(check_places(p));
   for (const void* s : {(const void*)p.lengths, (const void*)p.initial, (const void*)p.last}) TFFT_SEQ_CHECK(check_state(s));
   TFFT_SEQ_CHECK(check_workspace(p.workspace, p.workspace_bytes, workspace_of(p)));
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -201,6 +220,7 @@ extern "C" int tfft_scan_backward(const tfft_scan_grad_args* args, void* stream)
   TFFT_SEQ_CHECK(check_view(p.gate, p.gate_dtype, p.batch, p.length, p.channels / p.share, false));
   TFFT_SEQ_CHECK(check_view(p.dx, p.dtype, p.batch, p.length, p.channels, true));
   TFFT_SEQ_CHECK(check_view(p.dgate, p.gate_dtype, p.batch, p.length, p.channels / p.share, true));
+  if (p.length > 0) TFFT_SEQ_CHECK(check_places(p));
   for (const void* s : {(const void*)p.lengths, (const void*)p.initial, (const void*)p.dlast, (const void*)p.dinitial})
     TFFT_SEQ_CHECK(check_state(s));
   TFFT_SEQ_CHECK(check_workspace(p.workspace, p.workspace_bytes, workspace_of(p)));
@@ -225,6 +245,10 @@ extern "C" int tfft_scan_step(const tfft_scan_step_args* args, void* stream) {
   TFFT_SEQ_CHECK(check_view({(void*)p.state, p.state_batch, 0, 1}, TFFT_F32, p.batch, 1, p.channels, false));
   TFFT_SEQ_CHECK(check_view({p.new_state, p.new_state_batch, 0, 1}, TFFT_F32, p.batch, 1, p.channels, true));
   if (p.y) TFFT_SEQ_CHECK(check_view({p.y, p.y_batch, 0, 1}, p.dtype, p.batch, 1, p.channels, true));
+  if (same(p.new_state, p.x) || same(p.new_state, p.gate) || same(p.y, p.gate) || same(p.y, p.state) || same(p.y, p.new_state))
+    return refuse(who, "an output may not take another tensor's place");
+  if (p.batch > 1 && ((same(p.new_state, p.state) && p.new_state_batch != p.state_batch) || (same(p.y, p.x) && p.y_batch != p.x_batch)))
+    return refuse(who, "in place needs equal strides on both sides");
   if (p.batch * (p.channels + kRun) > kMaxExtent) return refuse(who, "more sequences than one launch takes");
   const unsigned runs = (unsigned)((p.channels + kRun - 1) / kRun), threads = (unsigned)p.batch * runs;
   hipStream_t s = static_cast<hipStream_t>(stream);

@@ -37,7 +37,7 @@ struct Chunking {
   long long state_words = 0;  // states of one chunk
   // 64-bit words: the counters, a map a state and chunk where groups are used, half a word a state and group
   long long words() const {
-    return apart() <= 1 ? 0 : kCounterWords * counters() + state_words * (group > 1 ? chunks : 0) +
+    return apart() <= 1 || tiles == 0 ? 0 : kCounterWords * counters() + state_words * (group > 1 ? chunks : 0) +
                                  (state_words * ((chunks + group - 1) / group) + 1) / 2;
   }
   long long apart() const { return walks ? 1 : chunks; }  // chunks that workgroups of their own take

@@ -274,10 +274,10 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void scan_rows_fwd(tfft_scan_arg
   if (!take_turn(f.turns, f.words, &lds.ticket, &tile, &chunk)) return;
   const Place at = place_of<V>(f, tile, lane);
   const int len = steps_of(p.lengths, at.b, f.length), t0 = (int)(chunk * waves + wave) * S;
-  const bool all = __all(t0 + S <= len && at.own == V);
+  const bool all = __all(t0 + S <= len && at.own == V), none = __all(t0 >= len);  // of the wave's steps lie inside
   Run<T, V> x[S];
   Run<G, VG> g[S];
-  if (f.length > 0) {
+  if (!none) {
     const int last = last_step(f, p.lengths, len);
     ask<S, V, STREAM>(Lane<T, Off>(p.x, at, at.c), t0, last, x);
     ask<S, VG, STREAM && VG == V>(Lane<G, Off>(p.gate, at, f.share == 1 ? at.c : at.c / f.share), t0, last, g);
@@ -354,11 +354,11 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void scan_rows_bwd(tfft_scan_gra
   const Place at = place_of<V>(f, tile, lane);
   const int len = steps_of(p.lengths, at.b, f.length);
   const int t0 = ((int)(f.chunks - 1 - chunk) * waves + (waves - 1 - wave)) * S;
-  const bool all = __all(t0 + S <= len && at.own == V);
+  const bool all = __all(t0 + S <= len && at.own == V), none = __all(t0 >= len);  // of the wave's steps lie inside
   const int gate = f.share == 1 ? at.c : at.c / f.share;
   Run<T, V> d[S], before[S];
   Run<G, VG> g[S];
-  if (f.length > 0) {
+  if (!none) {
     const int last = last_step(f, p.lengths, len);
     ask<S, V, STREAM>(Lane<T, Off>(p.dy, at, at.c), t0, last, d);
     ask<S, VG, STREAM && VG == V>(Lane<G, Off>(p.gate, at, gate), t0, last, g);
@@ -493,16 +493,20 @@ Shape shape_of(const P& p, const Chunking& c, int run, bool through, word* words
                p.gate_form == TFFT_GATE_LOG, (int)c.chunks, c.group, c.state_words, through ? 0u : (unsigned)(c.tiles / p.batch), turns_of(c), words};
 }
 
-bool gate_fits(const tfft_seq_view& gate, long long share, int run) { return share == 1 ? gate.channel == 1 : share % run == 0; }
+// Runs of neighbouring channels, all within 32 bits of the row's first one; a gate may be shared by whole runs
+bool runs_fit(long long channels, long long share, const tfft_seq_view& gate) {
+  return channels >= kRun && channels < (1LL << 28) &&
+         (share == 1 ? gate.channel == 1 : share % kRun == 0 && (__int128)(channels / share) * gate.channel < (1LL << 28));
+}
 
 }  // namespace
 
 bool rows_vector(const tfft_scan_args& p) {
-  return p.channels >= kRun && p.x.channel == 1 && p.y.channel == 1 && gate_fits(p.gate, p.share, kRun);
+  return runs_fit(p.channels, p.share, p.gate) && p.x.channel == 1 && p.y.channel == 1;
 }
 bool rows_vector(const tfft_scan_grad_args& p) {
-  return p.channels >= kRun && p.dy.channel == 1 && p.y.channel == 1 && p.dx.channel == 1 && gate_fits(p.gate, p.share, kRun) &&
-         (p.share > 1 || p.dgate.channel == 1);
+  return runs_fit(p.channels, p.share, p.gate) && p.dy.channel == 1 && p.y.channel == 1 && p.dx.channel == 1 &&
+         (p.share > 1 ? runs_fit(p.channels, p.share, p.dgate) : p.dgate.channel == 1);
 }
 
 static int run_of_call(const tfft_scan_args& p) { return rows_vector(p) ? kRun : 1; }

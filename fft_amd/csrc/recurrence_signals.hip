@@ -218,7 +218,7 @@ __global__ __launch_bounds__(64 * kMaxWaves<T>) void scan_signals_fwd(tfft_scan_
   if (!take<MODE>(f, lds, &row, &chunk)) return;
   const bool live = row < f.rows;
   if (!live) row = 0;
-  const int b = (int)(row / f.channels), c = (int)(row % f.channels), len = live ? steps_of(p.lengths, b, f.length) : 0;
+  const int b = (int)((unsigned)row / (unsigned)f.channels), c = (int)((unsigned)row - (unsigned)b * (unsigned)f.channels), len = live ? steps_of(p.lengths, b, f.length) : 0;
   const int order = threadIdx.x, piece = f.lanes < 64 ? order & (f.lanes - 1) : order;
   const int pieces = f.lanes < 64 ? f.lanes : (int)blockDim.x;
   const T* x = (const T*)p.x.data + b * p.x.batch + c * p.x.channel;
@@ -267,7 +267,7 @@ __global__ __launch_bounds__(64 * kMaxWaves<T>) void scan_signals_bwd(tfft_scan_
   if (!take<MODE>(f, lds, &row, &chunk)) return;
   const bool live = row < f.rows;
   if (!live) row = 0;
-  const int b = (int)(row / f.channels), c = (int)(row % f.channels), len = live ? steps_of(p.lengths, b, f.length) : 0;
+  const int b = (int)((unsigned)row / (unsigned)f.channels), c = (int)((unsigned)row - (unsigned)b * (unsigned)f.channels), len = live ? steps_of(p.lengths, b, f.length) : 0;
   const int order = threadIdx.x, piece = f.lanes < 64 ? order & (f.lanes - 1) : order;
   const int pieces = f.lanes < 64 ? f.lanes : (int)blockDim.x;
   const T* dy = (const T*)p.dy.data + b * p.dy.batch + c * p.dy.channel;

@@ -42,7 +42,7 @@ struct Grid {
   unsigned units, turned;  // of a head, and how many of them are rotated
   unsigned lanes;          // threads that share the heads of a token
   unsigned heads;          // of both tensors
-  unsigned long long threads;
+  unsigned threads;
 };
 
 template <class T>
@@ -64,19 +64,11 @@ __device__ __forceinline__ void put(T* to, const Run<T, R>& r, int valid) {
 template <class T, bool HALF, int NH, bool STREAM>
 __global__ __launch_bounds__(256) void rotary_units(tfft_rotary_args p, Grid g) {
   constexpr int R = kRun<T>, pairs = HALF ? R : R / 2;
-  const unsigned long long n = (unsigned long long)blockIdx.x * 256 + threadIdx.x;
+  const unsigned n = blockIdx.x * 256u + threadIdx.x;
   if (n >= g.threads) return;
-  const unsigned a_token = g.units * g.lanes;
-  long long token, b, t;
-  unsigned rest;
-  if (g.threads >> 32) {
-    token = (long long)(n / a_token), rest = (unsigned)(n - token * a_token);
-    b = token / p.length, t = token - b * p.length;
-  } else {
-    const unsigned i = (unsigned)n / a_token;
-    rest = (unsigned)n - i * a_token;
-    b = i / (unsigned)p.length, t = i - (unsigned)b * (unsigned)p.length;
-  }
+  const unsigned a_token = g.units * g.lanes, token = n / a_token, rest = n - token * a_token;
+  const unsigned entry = token / (unsigned)p.length;
+  const long long b = entry, t = token - entry * (unsigned)p.length;
   const unsigned hl = rest / g.units, u = rest - hl * g.units;
   const Token<T> first(p.tensor[0], b, t), second(p.tensor[1], b, t);
   const unsigned heads0 = (unsigned)p.tensor[0].heads;
@@ -137,7 +129,7 @@ __global__ __launch_bounds__(256) void rotary_units(tfft_rotary_args p, Grid g) 
 // Heads whose factors a thread shares: 8 x 4096 tokens with 32 + 8 heads of 128 in bf16 take 158, 130, 125, 126, 129 us with
 // 1, 2, 4, 5, 8. Calls that would be left with fewer than kEnough threads (256 CUs of 1024) give every head its own.
 constexpr int kHeads = 4;
-constexpr long long kEnough = 256 * 1024, kMost = 0x7fffffffLL;
+constexpr long long kEnough = 256 * 1024, kMost = 1LL << 30;
 
 int refuse(const char* why, int code = TFFT_ERR_INVALID) {
   char text[256];
@@ -157,7 +149,7 @@ extern "C" int tfft_rotary(const tfft_rotary_args* args, void* stream) {
   if (p.positions && p.position_bytes != 4 && p.position_bytes != 8) return refuse("position_bytes is 4 or 8");
   if (!p.turns) return refuse("no frequencies");
   if (!p.tensor[1].in) p.tensor[1].heads = 0;
-  if (p.batch > kMost || p.length > kMost || p.tensor[0].heads > kMost || p.tensor[1].heads > kMost)
+  if (p.batch > kMost || p.length > kMost || p.head > kMost || p.tensor[0].heads > kMost / 4 || p.tensor[1].heads > kMost / 4)
     return refuse("an extent is too large");
   // Results that leave in whole lines and whole units are streamed: 8 x 4096 tokens with 32 + 8 heads of 128 in bf16 119 us
   // against 126, 9003 tokens with 12 heads of 96 in fp32 15 against 17.
@@ -168,11 +160,18 @@ extern "C" int tfft_rotary(const tfft_rotary_args* args, void* stream) {
     const long long in[4] = {v.in_batch, v.in_time, v.in_head, 1}, out[4] = {v.out_batch, v.out_time, v.out_head, 1};
     if (const char* why = check_tensor(v.in, p.dtype, in, extent, false)) return refuse(why);
     if (const char* why = check_tensor(v.out, p.dtype, out, extent, true)) return refuse(why);
-    in_place = in_place && (v.heads == 0 || v.in == v.out);
+    if (v.heads == 0 || p.batch == 0 || p.length == 0) continue;
+    const bool here = v.in == v.out;
+    for (int i = 0; i < 3; ++i)
+      if (here && extent[i] > 1 && in[i] != out[i]) return refuse("in place needs equal strides on both sides");
+    in_place = in_place && here;
     const long long steps[3] = {v.out_batch, v.out_time, v.out_head}, counts[3] = {p.batch, p.length, v.heads};
-    stream_out = stream_out && (v.heads == 0 || whole_lines(v.out, p.dtype, steps, counts));
+    stream_out = stream_out && whole_lines(v.out, p.dtype, steps, counts);
   }
   const int run = p.dtype == TFFT_F32 ? kRun<float> : kRun<f16>;
+  const tfft_rotary_view &q = p.tensor[0], &k = p.tensor[1];
+  if (q.heads && k.heads && p.batch && p.length && (q.out == k.out || q.out == k.in || k.out == q.in))
+    return refuse("a result may not take the other tensor's place");
   Grid g;
   g.turned = ((p.pairs == TFFT_PAIRS_HALF ? p.rotary / 2 : p.rotary) + run - 1) / run;
   g.units = g.turned + (in_place ? 0 : (p.head - p.rotary + run - 1) / run);
@@ -182,9 +181,9 @@ extern "C" int tfft_rotary(const tfft_rotary_args* args, void* stream) {
   const bool many = (__int128)p.batch * p.length * g.units * g.heads >= (__int128)kHeads * kEnough;
   g.lanes = many ? (g.heads + kHeads - 1) / kHeads : g.heads;
   const __int128 threads = (__int128)p.batch * p.length * g.units * g.lanes;
-  if (threads > ((__int128)kMost << 8)) return refuse("more tokens and heads than one launch takes");
-  g.threads = (unsigned long long)threads;
-  const unsigned grid = (unsigned)((g.threads + 255) / 256);
+  if (threads > 0xffff0000LL) return refuse("more tokens and heads than one launch takes");
+  g.threads = (unsigned)threads;  // a launch counts its threads in 32 bits
+  const unsigned grid = (g.threads + 255) / 256;
   hipStream_t stream_ = static_cast<hipStream_t>(stream);
   const auto launch = [&](auto t) {
     using T = decltype(t);

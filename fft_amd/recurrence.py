@@ -30,6 +30,8 @@ def _placed(call, device, stream, *args):
     changes."""
     if stream is None and device == torch.cuda.current_device():
         return call(*args, torch._C._cuda_getCurrentRawStream(device))
+    if stream is not None and stream.device.index != device:
+        _refuse(f"{call.__name__.lstrip('_')}: the stream belongs to {stream.device}, the tensors to cuda:{device}")
     with torch.cuda.device(device):
         if stream is None:
             return call(*args, torch.cuda.current_stream(device).cuda_stream)

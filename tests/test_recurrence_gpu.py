@@ -320,3 +320,60 @@ def test_refusals():
         with pytest.raises(fft_amd.ThunderFFTError):
             call()
             print("not refused:", i)
+
+
+@pytest.mark.parametrize("dim,B,L,D,share", [(1, 40, 700, 330, 1), (1, 3, 1300, 4100, 1), (1, 2, 2000, 384, 48), (1, 3, 900, 640, 128),
+                                             (2, 9, 17000, 30, 1), (2, 40, 8211, 30, 1), (2, 2, 40000, 3, 1), (2, 1, 600000, 1, 1)])
+def test_larger(dim, B, L, D, share):
+    """Sizes at which tiles are dealt to the XCDs, rows are walked and chunks are taken apart, against the fp64
+    recurrence in torch on the device, by norms: the fp32 roundings of memories of up to 1000 steps, 4 of 2^-24 a
+    step, are 2.4e-4 at the very most, and random as they are a hundredth of that; 16-bit results add half a step."""
+    for dtype, gate_dtype in ((torch.float32, torch.float32), (torch.bfloat16, torch.float32), (torch.float16, torch.float16)):
+        x, gate, lengths, initial, dlast, dy = make(B, L, D, share, dtype, gate_dtype, dim, seed=L, ragged=True)
+        lengths[0] = L
+        y, last = recurrence.gated_scan(x, gate, dim=dim, log_gate=True, lengths=lengths, initial=initial)
+        got = recurrence.gated_scan_backward(dy, y, gate, dim=dim, log_gate=True, lengths=lengths, initial=initial, dlast=dlast)
+        rows = (lambda t: t.transpose(1, 2)) if dim == 1 else (lambda t: t)
+        inside = (torch.arange(L, device="cuda") < lengths[:, None])[:, None]
+        a = torch.where(inside, rows(gate).double().exp().repeat_interleave(share, 1), 1.0)
+
+        def run(a, v, h):  # [B, D, L] in stretches of 128 steps side by side, then joined
+            n = -(-L // 128)
+            pad = (0, n * 128 - L)
+            a = torch.nn.functional.pad(a, pad, value=1.0).view(B, D, n, 128)
+            v = torch.nn.functional.pad(v, pad).reshape(B, D, n, 128)
+            out, product = torch.empty_like(v), torch.cumprod(a, -1)
+            z = torch.zeros_like(v[..., 0])
+            for t in range(128):
+                z = a[..., t] * z + v[..., t]
+                out[..., t] = z
+            for j in range(n):
+                out[:, :, j] += product[:, :, j] * h[..., None]
+                h = out[:, :, j, -1]
+            return out.view(B, D, n * 128)[..., :L]
+
+        h = run(a, torch.where(inside, rows(x).double(), 0.0), initial.double())
+        later = torch.cat([a[..., 1:], torch.ones_like(a[..., :1])], -1)
+        e = run(later.flip(-1), torch.where(inside, rows(dy).double(), 0.0).flip(-1), dlast.double()).flip(-1)
+        before = torch.cat([initial.double()[..., None], rows(y).double()[..., :-1]], -1)
+        dgate = torch.where(inside, e * before * a, 0.0).reshape(B, D // share, share, L).sum(2)
+        for name, t, want in (("y", rows(y), torch.where(inside, h, 0.0)), ("last", last, h[..., -1]), ("dx", rows(got[0]), torch.where(inside, e, 0.0)),
+                              ("dgate", rows(got[1]), dgate), ("dinitial", got[2], a[..., 0] * e[..., 0])):
+            off = float((t.double() - want).norm() / want.norm())
+            assert off <= 2.4e-6 + torch.finfo(t.dtype).eps / 2, (name, dtype, off)
+            assert torch.isfinite(t).all(), name
+
+
+def test_places():
+    """Tensors at one address are taken element for element or refused."""
+    x, gate, _, _, _, dy = make(2, 50, 8, states=False)
+    y, _ = recurrence.gated_scan(x, gate)
+    square = torch.randn(2, 8, 8, device="cuda")
+    bad = [lambda: recurrence.gated_scan(x, gate, out=gate), lambda: recurrence.gated_scan(square, square.clone(), out=square.transpose(1, 2)),
+           lambda: recurrence.gated_scan_backward(dy, y, gate, dx=y), lambda: recurrence.gated_scan_backward(dy, y, gate, dx=gate),
+           lambda: recurrence.gated_scan_backward(dy, y, gate, dgate=gate), lambda: recurrence.gated_scan_backward(dy, y, gate, dgate=dy),
+           lambda: recurrence.gated_scan_step(x[:, 0], gate[:, 0], y[:, 0], out=y[:, 0])]
+    for i, call in enumerate(bad):
+        with pytest.raises(fft_amd.ThunderFFTError):
+            call()
+            print("not refused:", i)
