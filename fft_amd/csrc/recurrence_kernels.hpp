@@ -17,7 +17,8 @@
 // go round the XCDs): an XCD then reads whole rows, and lines that two tiles share once. B = 8, L = 4096 with D = 2048: 112 us forward
 // and 184 back, where the XCDs take every eighth tile 116 and 195; with D = 2050 120 and 219 against 140 and 251. With fewer than
 // kManyTiles tiles an eighth is too narrow, and all take from one counter, chunk by chunk: 65537 x 1152 (9 tiles) 129 us against
-// 197 with eight.
+// 197 with eight. In a padded batch an XCD has a strip of every entry instead, or the one with the longest sequences would be
+// the last to end (4 entries of up to 8191 steps, heads of 64: 94 us against 97 back).
 #pragma once
 #include "seq_common.hpp"
 
@@ -41,17 +42,23 @@ struct Chunking {
                                  (state_words * ((chunks + group - 1) / group) + 1) / 2;
   }
   long long apart() const { return walks ? 1 : chunks; }  // chunks that workgroups of their own take
+  long long strip = 0;  // neighbouring tiles of a counter, 0: an eighth of all
   int counters() const { return tiles >= kManyTiles ? 8 : 1; }
-  // workgroups; a few find no ticket left where the tiles do not divide evenly
-  long long blocks() const { return apart() <= 1 ? tiles : (tiles + counters() - 1) / counters() * counters() * chunks; }
+  long long width() const { return strip && counters() > 1 ? strip : (tiles + counters() - 1) / counters(); }
+  // workgroups: as many for every counter as the first one has tickets; a few find none left
+  long long blocks() const {
+    if (apart() <= 1) return tiles;
+    const long long round = counters() * width(), rest = tiles % round;
+    return counters() * (tiles / round * width() + (rest < width() ? rest : width())) * chunks;
+  }
 };
 
 // Tile and chunk of this workgroup, the same for all threads; false where there is none left. `shared` lies in LDS.
 struct Turns {
-  unsigned tiles, counters, chunks;
+  unsigned tiles, counters, chunks, width;
 };
 inline Turns turns_of(const Chunking& c) {
-  return Turns{(unsigned)c.tiles, (unsigned)c.counters(), (unsigned)c.apart()};
+  return Turns{(unsigned)c.tiles, (unsigned)c.counters(), (unsigned)c.apart(), (unsigned)c.width()};
 }
 __device__ __forceinline__ bool take_turn(const Turns& f, word* words, unsigned* shared, unsigned* tile, unsigned* chunk) {
   if (f.chunks <= 1) {
@@ -63,9 +70,12 @@ __device__ __forceinline__ bool take_turn(const Turns& f, word* words, unsigned*
     *shared = (unsigned)__hip_atomic_fetch_add(words + kCounterWords * counter, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
   const unsigned ticket = __builtin_amdgcn_readfirstlane(*shared);
-  const unsigned first = (unsigned)((word)counter * f.tiles / f.counters), mine = (unsigned)((word)(counter + 1) * f.tiles / f.counters) - first;
+  const unsigned round = f.counters * f.width, before = counter * f.width, rest = f.tiles % round;
+  const unsigned mine = f.tiles / round * f.width + min(rest > before ? rest - before : 0u, f.width);
+  if (mine == 0) return false;
   *chunk = __builtin_amdgcn_readfirstlane(ticket / mine);
-  *tile = first + (ticket - *chunk * mine);
+  const unsigned i = ticket - *chunk * mine;
+  *tile = i / f.width * round + before + i % f.width;
   return *chunk < f.chunks;
 }
 

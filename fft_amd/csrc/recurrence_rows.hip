@@ -469,7 +469,7 @@ bool through_batch(int run, long long batch, long long channels, std::initialize
   return true;
 }
 
-Chunking plan(long long batch, long long length, long long channels, int run, bool through, int steps) {
+Chunking plan(long long batch, long long length, long long channels, int run, bool through, int steps, bool padded_batch) {
   Chunking c;
   const long long padded = (channels + run - 1) / run * run, width = 64 * run;
   c.tiles = through ? (batch * padded + width - 1) / width : batch * ((channels + width - 1) / width);
@@ -479,6 +479,7 @@ Chunking plan(long long batch, long long length, long long channels, int run, bo
   c.waves = (int)((pieces + c.chunks - 1) / c.chunks);
   c.chunks = (pieces + c.waves - 1) / c.waves;
   c.state_words = c.tiles * width;
+  if (padded_batch) c.strip = c.tiles / (8 * batch) > 1 ? c.tiles / (8 * batch) : 1;
   // About kResident workgroups run at once, kResident / tiles chunks of each tile. That many are joined directly, so that few
   // channels wait for one state in that many chunks, and many channels do not read what they need not: B = 8,
   // L = 4096, D = 2048 (128 tiles) takes 118, 121, 129 us with groups of 4, 8, 16; one sequence of 65537 steps
@@ -518,10 +519,10 @@ static bool through_batch(const tfft_scan_grad_args& p) {
   return through_batch(run_of_call(p), p.batch, p.channels, {&p.dy, &p.y, &p.gate, &p.dx, &p.dgate});
 }
 Chunking plan_rows(const tfft_scan_args& p) {
-  return plan(p.batch, p.length, p.channels, run_of_call(p), through_batch(p), kStepsForward);
+  return plan(p.batch, p.length, p.channels, run_of_call(p), through_batch(p), kStepsForward, p.lengths != nullptr);
 }
 Chunking plan_rows(const tfft_scan_grad_args& p) {
-  return plan(p.batch, p.length, p.channels, run_of_call(p), through_batch(p), steps_backward(p.dtype));
+  return plan(p.batch, p.length, p.channels, run_of_call(p), through_batch(p), steps_backward(p.dtype), p.lengths != nullptr);
 }
 
 // Lanes that share a gate, where whole power-of-two groups of a wave's lanes do; 0: summed by a kernel of its own

@@ -322,12 +322,13 @@ __global__ __launch_bounds__(64 * kMaxWaves<T>) void scan_signals_bwd(tfft_scan_
   if (p.dinitial && live && chunk + 1 == (unsigned)f.chunks && piece == pieces - 1) p.dinitial[row] = k;
 }
 
-Chunking plan(long long batch, long long length, long long channels, int dtype) {
+Chunking plan(long long batch, long long length, long long channels, int dtype, bool padded_batch) {
   const int steps = dtype == TFFT_F32 ? kSteps<float> : kSteps<f16>, most = dtype == TFFT_F32 ? kMaxWaves<float> : kMaxWaves<f16>;
   Chunking c;
   const long long rows = batch * channels, pieces = (length + steps - 1) / steps;
   c.tiles = rows;
   c.state_words = rows;
+  c.strip = padded_batch;
   c.group = kMaxGroup;
   if (pieces <= 32) {
     c.lanes = 1;
@@ -363,8 +364,8 @@ bool signals_fit(const tfft_scan_args& p) {
 bool signals_fit(const tfft_scan_grad_args& p) {
   return p.share == 1 && p.dy.time == 1 && p.y.time == 1 && p.dx.time == 1 && p.dgate.time == 1 && p.gate.time <= 1;
 }
-Chunking plan_signals(const tfft_scan_args& p) { return plan(p.batch, p.length, p.channels, p.dtype); }
-Chunking plan_signals(const tfft_scan_grad_args& p) { return plan(p.batch, p.length, p.channels, p.dtype); }
+Chunking plan_signals(const tfft_scan_args& p) { return plan(p.batch, p.length, p.channels, p.dtype, p.lengths != nullptr); }
+Chunking plan_signals(const tfft_scan_grad_args& p) { return plan(p.batch, p.length, p.channels, p.dtype, p.lengths != nullptr); }
 
 void launch_signals(const tfft_scan_args& p, const Chunking& c, word* words, hipStream_t s) {
   const Shape f = shape_of(p, c, words);
