@@ -30,6 +30,9 @@ __device__ __forceinline__ void turn(uint64_t phase, float* c, float* s) {
   }
 }
 
+// What bounds it: HBM. 8 x 4096 tokens with 32 + 8 heads of 128 in bf16 take 118 us (671 MB, 5.7 TB/s); the factors, evaluated in
+// registers from 8 bytes a pair, hide behind it. One token each of 64 sequences takes 4 us, a launch and its latency.
+//
 // A unit is what a thread holds of one head: kRun<T> values (16 bytes) of each half (pairs i, i + rotary / 2), twice as many
 // pairs, or kRun<T> values with their kRun<T> / 2 interleaved pairs; behind the rotated ones, kRun<T> values to copy.
 template <class T>
