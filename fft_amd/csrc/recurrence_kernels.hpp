@@ -47,7 +47,7 @@ struct Chunking {
   long long width() const { return strip && counters() > 1 ? strip : (tiles + counters() - 1) / counters(); }
   // workgroups: as many for every counter as the first one has tickets; a few find none left
   long long blocks() const {
-    if (apart() <= 1) return tiles;
+    if (apart() <= 1 || tiles == 0) return tiles;
     const long long round = counters() * width(), rest = tiles % round;
     return counters() * (tiles / round * width() + (rest < width() ? rest : width())) * chunks;
   }

@@ -487,7 +487,7 @@ Chunking plan(long long batch, long long length, long long channels, int run, bo
   c.waves = (int)((pieces + c.chunks - 1) / c.chunks);
   c.chunks = (pieces + c.waves - 1) / c.waves;
   c.state_words = c.tiles * width;
-  if (padded_batch) c.strip = c.tiles / (8 * batch) > 1 ? c.tiles / (8 * batch) : 1;
+  if (padded_batch && batch > 0) c.strip = c.tiles / (8 * batch) > 1 ? c.tiles / (8 * batch) : 1;
   // About kResident workgroups run at once, kResident / tiles chunks of each tile. That many are joined directly, so that few
   // channels wait for one state in that many chunks, and many channels do not read what they need not: B = 8,
   // L = 4096, D = 2048 (128 tiles) takes 118, 121, 129 us with groups of 4, 8, 16; one sequence of 65537 steps

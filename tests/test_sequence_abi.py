@@ -21,12 +21,12 @@ def scan(dtype=BF16, gate_dtype=F32, form=1, B=2, L=100, D=64, share=1, x=None, 
 
 
 def grad(dtype=BF16, gate_dtype=F32, form=1, B=2, L=100, D=64, share=1, views=None, size=_lib.SCAN_GRAD_ARGS.size, workspace=A,
-         workspace_bytes=1 << 40):
+         workspace_bytes=1 << 40, lengths=0):
     G = D // share
     wide, narrow = (L * D, D, 1), (L * G, G, 1)
     views = views or [(A, *wide), (2 * A, *wide), (3 * A, *narrow), (4 * A, *wide), (5 * A, *narrow)]
     flat = [v for view in views for v in view]
-    return _lib.SCAN_GRAD_ARGS.pack(size, dtype, gate_dtype, form, B, L, D, share, *flat, 0, 0, 0, A, workspace, workspace_bytes)
+    return _lib.SCAN_GRAD_ARGS.pack(size, dtype, gate_dtype, form, B, L, D, share, *flat, lengths, 0, 0, A, workspace, workspace_bytes)
 
 
 def step(dtype=BF16, gate_dtype=F32, form=1, B=2, D=64, share=1, places=(A, 2 * A, 3 * A, 3 * A, 4 * A), strides=None,
@@ -128,6 +128,14 @@ def test_nothing_to_do():
     assert lib.tfft_scan_step(step(B=0), None) == OK
     assert lib.tfft_rotary(rotary(B=0), None) == OK and lib.tfft_rotary(rotary(L=0), None) == OK
     assert lib.tfft_rotary(rotary(views=((0, 0, 0) + VIEW[3:], (0,) * 9)), None) == OK
+
+
+@pytest.mark.parametrize("empty", [dict(B=0), dict(B=0, L=0), dict(B=0, L=9000), dict(D=0)])
+def test_an_empty_padded_batch(empty):
+    lib = _lib.load()
+    assert workspace(scan(lengths=A, **empty)) == (OK, 0) and lib.tfft_scan_forward(scan(lengths=A, **empty), None) == OK
+    back = grad(lengths=A, **empty)
+    assert workspace(backward=back) == (OK, 0) and lib.tfft_scan_backward(back, None) == OK
 
 
 def test_workspaces():
