@@ -156,7 +156,7 @@ extern "C" int tfft_rotary(const tfft_rotary_args* args, void* stream) {
     return refuse("an extent is too large");
   // Results that leave in whole lines and whole units are streamed: 8 x 4096 tokens with 32 + 8 heads of 128 in bf16 119 us
   // against 126, 9003 tokens with 12 heads of 96 in fp32 15 against 17.
-  const int size = p.dtype == TFFT_F32 ? 4 : 2;
+  const long long size = p.dtype == TFFT_F32 ? 4 : 2;
   bool in_place = true, stream_out = p.rotary / 2 * size % 16 == 0 && p.head * size % 16 == 0;
   for (const tfft_rotary_view& v : p.tensor) {
     const long long extent[4] = {p.batch, p.length, v.heads, p.head};

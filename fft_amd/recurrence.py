@@ -123,7 +123,7 @@ def gated_scan(x, gate, dim=1, log_gate=False, lengths=None, initial=None, out=N
 
     x: [B, L, D] (dim = 1) or [B, D, L] (dim = 2), float32, float16 or bfloat16, any strides. gate: the same with G
     channels, one for D / G neighbours, of x's type or float32; with log_gate the decay is exp(gate). lengths (int32
-    [B]): steps behind a sequence's length are not read, leave the state as it is, and y is 0 there. initial: fp32
+    [B]): steps behind a sequence's length do not count, leave the state as it is, and y is 0 there. initial: fp32
     [B, D]. out: a tensor for y, x itself allowed. Asynchronous on `stream` (default: torch's current stream)."""
     return _placed(_gated_scan, _same_device("gated_scan", x, gate, lengths, initial, out), stream, x, gate, dim, log_gate,
                    lengths, initial, out)

@@ -302,9 +302,10 @@ int tfft_get_twiddle_table(int dtype, int n, const void** d_table);
  * Element types: x, y and their gradients have `dtype`; the gate has `gate_dtype`, TFFT_F32 or `dtype`. States
  * (initial, last and their gradients) are contiguous fp32 [batch][channels]; all arithmetic is fp32 and every output is
  * rounded once. gate_form TFFT_GATE_DECAY: a = gate; TFFT_GATE_LOG: a = exp(gate), a gate of minus infinity restarts
- * the recurrence. `share` consecutive channels share one gate: the gate has channels / share entries a step (share
- * divides channels). |a| <= 1 is what the operator is made for; larger decays are computed as long as the product of
- * the decays over the sequence stays finite in fp32.
+ * the recurrence, whatever finite state it has (like a decay of 0; 0 times infinity is NaN). `share` consecutive
+ * channels share one gate: the gate has channels / share entries a step (share divides channels). |a| <= 1 is what the
+ * operator is made for; larger decays are computed as long as the product of the decays over the sequence stays finite
+ * in fp32.
  *
  * Layout: element strides (batch, time, channel; for the gate: batch, time, gate). Any non-negative strides are taken;
  * inputs may repeat (stride 0), outputs may not. Layouts with kernels of their own are channel stride 1 ([batch][time]
@@ -312,7 +313,7 @@ int tfft_get_twiddle_table(int dtype, int n, const void** d_table);
  * dx) may be the same buffer with the same strides; every other overlap of an output with anything gives wrong results.
  *
  * lengths (NULL, or int32 [batch] on the device, clamped to 0 ... length): a padded batch. The steps behind a
- * sequence's length leave its state as it is and are not read (NaN there does no harm); y, dx and dgate are 0 there.
+ * sequence's length leave its state as it is and do not count (NaN there does no harm); y, dx and dgate are 0 there.
  * A sequence of length 0 has last = initial.
  *
  * Results do not depend on timing: the same call gives the same bits. Asynchronous on `stream`; allocates nothing.
