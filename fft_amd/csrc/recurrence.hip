@@ -8,10 +8,10 @@ using namespace tfft_seq;
 // The words that chunks hand their states on with, cleared by a kernel of the same call: it may be captured and
 // replayed, and nothing of an earlier call is left in them.
 __global__ __launch_bounds__(256) void clear_words(word* words, long long n) {
-  const long long at = 4 * ((long long)blockIdx.x * 256 + threadIdx.x);
+  const long long first = 1024ll * blockIdx.x + threadIdx.x;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (at + i < n) words[at + i] = 0;
+    if (first + 256 * i < n) words[first + 256 * i] = 0;
 }
 
 // One token: a thread has kRun neighbouring channels of a row. What counts is latency (a full batch of 512 x 4096 channels is 29 MB,
