@@ -52,38 +52,7 @@ __device__ __forceinline__ Run<G, E> one(const G* p) {
 template <int E, class T>
 __device__ __forceinline__ void line_up(Run<T, E>& r, int t0, int length) {
   const int by = length < E ? 0 : min(max(t0 - (length - E), 0), E);  // steps that the run starts too early
-  if (__all(by == 0)) return;
-  constexpr int kWords = sizeof(r.w) / 4, kElements = 4 / sizeof(T);
-#pragma unroll
-  for (int m = kWords; m >= 1; m /= 2) {
-    const bool move = by / kElements & m;
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) r.w[i] = move ? (i + m < kWords ? r.w[i + m] : 0u) : r.w[i];
-  }
-  if constexpr (kElements == 2) {
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) r.w[i] = by & 1 ? r.w[i] >> 16 | (i + 1 < kWords ? r.w[i + 1] << 16 : 0u) : r.w[i];
-  }
-}
-// The first `valid` of E elements, fewer than E: halves, quarters and so on as the bits of `valid` say, what follows moved down
-template <int N, class T, int E>
-__device__ __forceinline__ void store_head(T* p, Run<T, E> r, int valid) {
-  if constexpr (N > 1) {
-    constexpr int kWords = N / 2 * sizeof(T) / 4;  // of the half; 0: half a word
-    if (valid & (N / 2)) {
-      if constexpr (kWords == 0) {
-        Run<T, 1> one;
-        one.w[0] = r.w[0];
-        store_run<T, 1>(p, one);
-      } else {
-        __builtin_memcpy(p, r.w, 4 * kWords);
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) r.w[i] = r.w[i + kWords];
-      }
-      p += N / 2;
-    }
-    store_head<N / 2>(p, r, valid);
-  }
+  move_down<E>(r, by);
 }
 // STREAM: as in load_run. Two stores share a line here, which costs a row in one workgroup 1 to 8 %, but where chunks are taken apart the
 // states come through faster: two entries of 8 signals of 1048573 steps in fp32 take 47 us forward and 74 back against 53 and 90.

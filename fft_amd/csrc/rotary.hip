@@ -33,10 +33,14 @@ __device__ __forceinline__ void turn(uint64_t phase, float* c, float* s) {
 // What bounds it: HBM. 8 x 4096 tokens with 32 + 8 heads of 128 in bf16 take 118 us (671 MB, 5.7 TB/s); the factors, evaluated in
 // registers from 8 bytes a pair, hide behind it. One token each of 64 sequences takes 4 us, a launch and its latency.
 //
-// A unit is what a thread holds of one head: kRun<T> values (16 bytes) of each half (pairs i, i + rotary / 2), twice as many
-// pairs, or kRun<T> values with their kRun<T> / 2 interleaved pairs; behind the rotated ones, kRun<T> values to copy.
+// A unit is what a thread holds of one head: R values of each half (pairs i, i + rotary / 2), twice as many pairs, or R values
+// with their R / 2 interleaved pairs; behind the rotated ones, R values to copy. R is kRun<T> (16 bytes), or kShortRun in heads
+// that have fewer values. A unit that reaches over the end of the head is loaded as the head's last R values and moved to where it
+// belongs: all loads are whole runs on one path, because one whose registers two paths could fill is waited for where they meet
+// (5 x 2489 tokens with 21 heads of 174 in fp16 take 49 us, 76 when the last units are loaded value by value).
 template <class T>
 constexpr int kRun = 16 / sizeof(T);
+constexpr int kShortRun = 2;
 
 // A thread evaluates the factors of its unit once and turns it in the heads hl, hl + lanes, ... of its token, the second
 // tensor's heads counted behind the first's. Neighbouring threads have neighbouring units, then neighbouring heads: a wave
@@ -61,12 +65,13 @@ struct Token {
 template <int R, bool STREAM, class T>
 __device__ __forceinline__ void put(T* to, const Run<T, R>& r, int valid) {
   if constexpr (STREAM) store_run<T, R, true>(to, r);  // all units are whole
-  else store_some<R>(to, r, valid);
+  else if (valid == R) store_run<T, R>(to, r);
+  else store_head<R>(to, r, valid);
 }
 
-template <class T, bool HALF, int NH, bool STREAM>
+template <class T, bool HALF, int R, int NH, bool STREAM>
 __global__ __launch_bounds__(256) void rotary_units(tfft_rotary_args p, Grid g) {
-  constexpr int R = kRun<T>, pairs = HALF ? R : R / 2;
+  constexpr int pairs = HALF ? R : R / 2;
   const unsigned n = blockIdx.x * 256u + threadIdx.x;
   if (n >= g.threads) return;
   const unsigned a_token = g.units * g.lanes, token = n / a_token, rest = n - token * a_token;
@@ -80,6 +85,9 @@ __global__ __launch_bounds__(256) void rotary_units(tfft_rotary_args p, Grid g) 
   // where the unit's values lie in the head, and how many of them are there
   const int at = turned ? (int)u * R : p.rotary + (int)(u - g.turned) * R;
   const int valid = min(R, turned ? (HALF ? half - at : p.rotary - at) : p.head - at);
+
+  // where the unit's runs are loaded, and how many values too early
+  const int from_x = min(at, p.head - R), from_y = min(at + half, p.head - R);
 
   float c[pairs], s[pairs];
   if (turned) {
@@ -103,16 +111,18 @@ __global__ __launch_bounds__(256) void rotary_units(tfft_rotary_args p, Grid g) 
       if (h < g.heads) {
         const bool one = h < heads0;
         const long long i = one ? h : h - heads0;
-        const T* from = (one ? first.in + i * first.in_head : second.in + i * second.in_head) + at;
+        const T* from = one ? first.in + i * first.in_head : second.in + i * second.in_head;
         to[j] = (one ? first.out + i * first.out_head : second.out + i * second.out_head) + at;
-        x[j] = load_some<R>(from, valid);
-        if (HALF && turned) y[j] = load_some<R>(from + half, valid);
+        x[j] = load_run<T, R>(from + from_x);
+        if (HALF && turned) y[j] = load_run<T, R>(from + from_y);
       }
     }
 #pragma unroll
     for (int j = 0; j < NH; ++j) {
       if (h0 + j * g.lanes >= g.heads) continue;
+      move_down<R>(x[j], at - from_x);
       if (turned) {
+        if (HALF) move_down<R>(y[j], at + half - from_y);
         Run<T, R> re, im;
 #pragma unroll
         for (int k = 0; k < pairs; ++k) {
@@ -171,7 +181,7 @@ extern "C" int tfft_rotary(const tfft_rotary_args* args, void* stream) {
     const long long steps[3] = {v.out_batch, v.out_time, v.out_head}, counts[3] = {p.batch, p.length, v.heads};
     stream_out = stream_out && whole_lines(v.out, p.dtype, steps, counts);
   }
-  const int run = p.dtype == TFFT_F32 ? kRun<float> : kRun<f16>;
+  const int whole = p.dtype == TFFT_F32 ? kRun<float> : kRun<f16>, run = p.head < whole ? kShortRun : whole;
   const tfft_rotary_view &q = p.tensor[0], &k = p.tensor[1];
   if (q.heads && k.heads && p.batch && p.length && (q.out == k.out || q.out == k.in || k.out == q.in))
     return refuse("a result may not take the other tensor's place");
@@ -181,7 +191,7 @@ extern "C" int tfft_rotary(const tfft_rotary_args* args, void* stream) {
   g.heads = (unsigned)(p.tensor[0].heads + p.tensor[1].heads);
   if (p.batch == 0 || p.length == 0 || g.heads == 0) return TFFT_OK;
   // kHeads heads a thread share its factors where that leaves enough threads to fill the chip, else one
-  const bool many = (__int128)p.batch * p.length * g.units * g.heads >= (__int128)kHeads * kEnough;
+  const bool many = run != kShortRun && (__int128)p.batch * p.length * g.units * g.heads >= (__int128)kHeads * kEnough;
   g.lanes = many ? (g.heads + kHeads - 1) / kHeads : g.heads;
   const __int128 threads = (__int128)p.batch * p.length * g.units * g.lanes;
   if (threads > 0xffff0000LL) return refuse("more tokens and heads than one launch takes");
@@ -191,9 +201,10 @@ extern "C" int tfft_rotary(const tfft_rotary_args* args, void* stream) {
   const auto launch = [&](auto t) {
     using T = decltype(t);
     const auto pairs = [&](auto half) {
-      if (!many) rotary_units<T, half.value, 1, false><<<grid, 256, 0, stream_>>>(p, g);
-      else if (stream_out) rotary_units<T, half.value, kHeads, true><<<grid, 256, 0, stream_>>>(p, g);
-      else rotary_units<T, half.value, kHeads, false><<<grid, 256, 0, stream_>>>(p, g);
+      if (run == kShortRun) rotary_units<T, half.value, kShortRun, 1, false><<<grid, 256, 0, stream_>>>(p, g);
+      else if (!many) rotary_units<T, half.value, kRun<T>, 1, false><<<grid, 256, 0, stream_>>>(p, g);
+      else if (stream_out) rotary_units<T, half.value, kRun<T>, kHeads, true><<<grid, 256, 0, stream_>>>(p, g);
+      else rotary_units<T, half.value, kRun<T>, kHeads, false><<<grid, 256, 0, stream_>>>(p, g);
     };
     if (p.pairs == TFFT_PAIRS_HALF) pairs(std::true_type());
     else pairs(std::false_type());
