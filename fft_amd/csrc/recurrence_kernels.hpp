@@ -32,14 +32,17 @@ struct Chunking {
   long long tiles = 0;   // rows: groups of channels; signals: groups of rows
   long long chunks = 0;  // of the time axis
   int waves = 0;         // of a workgroup
-  int group = 1;         // chunks whose (A, B) are joined directly; the state behind each group is handed on
+  int group = 1;         // chunks whose (A, B) are joined directly
+  int row = 1;           // groups whose (A, B) are joined directly; the state behind each row of groups is handed on
   int lanes = 64;        // signals: threads of a row, where a wave holds several rows
   bool walks = false;    // a workgroup takes all chunks of its tile, one after the other
   long long state_words = 0;  // states of one chunk
-  // 64-bit words: the counters, a map a state and chunk where groups are used, half a word a state and group
+  // 64-bit words: the counters, a map a state and chunk where groups are used and a group where rows of them are, half a word a
+  // state and row
   long long words() const {
-    return apart() <= 1 || tiles == 0 ? 0 : kCounterWords * counters() + state_words * (group > 1 ? chunks : 0) +
-                                 (state_words * ((chunks + group - 1) / group) + 1) / 2;
+    if (apart() <= 1 || tiles == 0) return 0;
+    const long long groups = (chunks + group - 1) / group, rows = (groups + row - 1) / row;
+    return kCounterWords * counters() + state_words * ((group > 1 ? chunks : 0) + (row > 1 ? groups : 0)) + (state_words * rows + 1) / 2;
   }
   long long apart() const { return walks ? 1 : chunks; }  // chunks that workgroups of their own take
   long long strip = 0;  // neighbouring tiles of a counter, 0: an eighth of all

@@ -33,7 +33,7 @@ using offset_of = std::conditional_t<V == 1, long long, uint32_t>;
 struct Shape {
   int batch, length, channels, padded;  // padded: channels rounded up to whole runs
   int share, log_gate;
-  int chunks, group;
+  int chunks, group, row;
   long long state_words;
   unsigned tiles_of_entry;  // 0: tiles run through the whole batch
   Turns turns;
@@ -105,57 +105,74 @@ __device__ __forceinline__ void store_state(float* to, const Place& p, int chann
     if (v >= V - p.own) to[(long long)p.b * channels + p.c + v] = h[v];
 }
 
-// The state in front of this chunk, for the wave that has the (A, B) of the whole chunk, from the words of earlier chunks (or
-// `start`, in front of the first). Publishes this chunk's own words on the way. The maps of the group are joined while the state
-// behind the group before is still on its way, so that it is handed on at once when it comes.
+// The joint map of `count` maps that follow one another, `step` words apart, as soon as they are there
 template <int V>
-__device__ __forceinline__ void state_before(const Shape& f, const float* start, const Place& at, unsigned chunk, const float (&A)[V],
-                                             const float (&B)[V], float (&h)[V]) {
-  word* maps = f.words + kCounterWords * f.turns.counters;
-  unsigned* states = (unsigned*)(maps + (f.group > 1 ? f.state_words * f.chunks : 0));
-  const int r = chunk % f.group, q = chunk / f.group;
-  const bool more = chunk + 1 < (unsigned)f.chunks;
-  if (more && r != f.group - 1) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) publish_map(maps + f.state_words * chunk + at.n + v, A[v], B[v]);
-  }
-  float a[V], b[V];
+__device__ __forceinline__ void join_words(const word* from, long long step, int count, float (&a)[V], float (&b)[V]) {
 #pragma unroll
   for (int v = 0; v < V; ++v) a[v] = 1.0f, b[v] = 0.0f;
   constexpr int kAtOnce = 4;
 #pragma unroll 1
-  for (int k = 0; k < r; k += kAtOnce) {
+  for (int k = 0; k < count; k += kAtOnce, from += kAtOnce * step) {
     word w[kAtOnce][V];
-    const word* from = maps + f.state_words * (chunk - r + k) + at.n;
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i)
 #pragma unroll
-      for (int v = 0; v < V; ++v) w[i][v] = peek(from + (k + i < r ? f.state_words * i : 0) + v);
+      for (int v = 0; v < V; ++v) w[i][v] = peek(from + (k + i < count ? step * i : 0) + v);
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
-      if (k + i >= r) break;
+      if (k + i >= count) break;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        if (!w[i][v]) w[i][v] = await(from + f.state_words * i + v);
+        if (!w[i][v]) w[i][v] = await(from + step * i + v);
         b[v] = join(map_a(w[i][v]), b[v], map_b(w[i][v]));
         a[v] *= map_a(w[i][v]);
       }
     }
   }
-  if (q == 0) {
+}
+
+// The state in front of this chunk, for the wave that has the (A, B) of the whole chunk, from the words of earlier chunks (or
+// `start`, in front of the first): the maps of its group's chunks before it, those of the groups before it in their row of
+// groups, and the state in front of that row. Publishes this chunk's own words on the way, each as soon as it is known.
+template <int V>
+__device__ __forceinline__ void state_before(const Shape& f, const float* start, const Place& at, unsigned chunk, const float (&A)[V],
+                                             const float (&B)[V], float (&h)[V]) {
+  const int r = chunk % f.group, q = chunk / f.group, u = q % f.row, s = q / f.row;
+  const bool more = chunk + 1 < (unsigned)f.chunks, last = r == f.group - 1;
+  word* maps = f.words + kCounterWords * f.turns.counters + at.n;
+  word* of_groups = maps + (f.group > 1 ? f.state_words * f.chunks : 0);
+  unsigned* states = (unsigned*)(of_groups - at.n + (f.row > 1 ? f.state_words * ((f.chunks + f.group - 1) / f.group) : 0)) + at.n;
+  if (more && !last) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) publish_map(maps + f.state_words * chunk + v, A[v], B[v]);
+  }
+  float a[V], b[V];
+  join_words<V>(maps + f.state_words * (chunk - r), f.state_words, r, a, b);
+  if (f.row > 1) {
+    if (more && last && u != f.row - 1) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) publish_map(of_groups + f.state_words * q + v, A[v] * a[v], join(A[v], b[v], B[v]));
+    }
+    float ga[V], gb[V];
+    join_words<V>(of_groups + f.state_words * (q - u), f.state_words, u, ga, gb);
+#pragma unroll
+    for (int v = 0; v < V; ++v) b[v] = join(a[v], gb[v], b[v]), a[v] *= ga[v];
+  }
+  if (s == 0) {
     load_state<V>(start, at, f.channels, h);
   } else {
     unsigned w[V];
+    const unsigned* from = states + f.state_words * (s - 1);
 #pragma unroll
-    for (int v = 0; v < V; ++v) w[v] = peek(states + f.state_words * (q - 1) + at.n + v);
+    for (int v = 0; v < V; ++v) w[v] = peek(from + v);
 #pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = __uint_as_float(w[v] ? w[v] : await(states + f.state_words * (q - 1) + at.n + v));
+    for (int v = 0; v < V; ++v) h[v] = __uint_as_float(w[v] ? w[v] : await(from + v));
   }
 #pragma unroll
   for (int v = 0; v < V; ++v) h[v] = join(a[v], h[v], b[v]);
-  if (more && r == f.group - 1) {
+  if (more && last && u == f.row - 1) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) publish_state(states + f.state_words * q + at.n + v, join(A[v], h[v], B[v]));
+    for (int v = 0; v < V; ++v) publish_state(states + f.state_words * s + v, join(A[v], h[v], B[v]));
   }
 }
 
@@ -493,13 +510,16 @@ Chunking plan(long long batch, long long length, long long channels, int run, bo
   // L = 4096, D = 2048 (128 tiles) takes 118, 121, 129 us with groups of 4, 8, 16; one sequence of 65537 steps
   // and 1024 channels (8 tiles) 180, 129, 119 us.
   while (c.group < kMaxGroup && c.group * c.tiles < kResident) c.group *= 2;
+  // With one or two tiles the states of one group after the other are what a call waits for: one sequence of 65537 steps in bf16 takes
+  // 39, 46 us with 128, 256 channels so, 24, 36 in rows of groups; with 1024 channels 96 against 102.
+  if (c.tiles <= 2) c.row = kMaxGroup;
   return c;
 }
 
 template <class P>
 Shape shape_of(const P& p, const Chunking& c, int run, bool through, word* words) {
   return Shape{(int)p.batch, (int)p.length, (int)p.channels, (int)((p.channels + run - 1) / run * run), (int)p.share,
-               p.gate_form == TFFT_GATE_LOG, (int)c.chunks, c.group, c.state_words, through ? 0u : (unsigned)(c.tiles / p.batch), turns_of(c), words};
+               p.gate_form == TFFT_GATE_LOG, (int)c.chunks, c.group, c.row, c.state_words, through ? 0u : (unsigned)(c.tiles / p.batch), turns_of(c), words};
 }
 
 // Runs of neighbouring channels, all within 32 bits of the row's first one; a gate may be shared by whole runs

@@ -15,10 +15,12 @@ namespace {
 // cost up to a quarter (L = 4095 in bf16 123 us against 103).
 constexpr int kMaxGroup = 64;
 // Longer rows that are many are walked by a workgroup each, chunk after chunk, few rows are split: 256 x 20000 in bf16 takes 11 us
-// walked against 13 split, 256 x 100000 in fp32 65 against 69, 16 x 2^20 47 split (16 workgroups would walk). From kShortChunks
+// walked against 13 split, 256 x 100000 in fp32 65 against 69, 16 x 2^20 47 split (16 workgroups would walk). Back in 16 bits
+// a few hundred workgroups, two on some CUs and one on the others, last longer: 294 x 52347 in bf16 61 us walked against 39
+// split, 500 x 60000 71 against 64 (in fp32 300 x 30000 43 against 46). From kShortChunks
 // rows on the workgroups have 4 waves, and several of a CU load, wait and store at different times: 49152 x 8200 in bf16 449 us
 // forward and 769 back against 657 and 1351 with 8 waves; with 256 rows they are too few, 96 and 125 us against 65 and 110.
-constexpr int kManyRows = 256, kShortChunks = 1024, kWalkWaves = 4;
+constexpr int kManyRows = 256, kManyRowsBack = 512, kShortChunks = 1024, kWalkWaves = 4;
 enum { ONE, WALK, SPLIT };  // one chunk, or chunks after one another, or apart
 template <class T>
 constexpr int kSteps = 32 / sizeof(T);
@@ -297,7 +299,7 @@ __global__ __launch_bounds__(64 * kMaxWaves<T>) void scan_signals_bwd(tfft_scan_
   if (p.dinitial && live && chunk + 1 == (unsigned)f.chunks && piece == pieces - 1) p.dinitial[row] = k;
 }
 
-Chunking plan(long long batch, long long length, long long channels, int dtype, bool padded_batch) {
+Chunking plan(long long batch, long long length, long long channels, int dtype, bool padded_batch, int many) {
   const int steps = dtype == TFFT_F32 ? kSteps<float> : kSteps<f16>, most = dtype == TFFT_F32 ? kMaxWaves<float> : kMaxWaves<f16>;
   Chunking c;
   const long long rows = batch * channels, pieces = (length + steps - 1) / steps;
@@ -312,7 +314,7 @@ Chunking plan(long long batch, long long length, long long channels, int dtype, 
     c.chunks = 1;
     return c;
   }
-  c.walks = pieces > 64 * most && rows >= kManyRows;
+  c.walks = pieces > 64 * most && rows >= many;
   const int waves = c.walks && rows >= kShortChunks ? kWalkWaves : most;
   c.chunks = (pieces + 64 * waves - 1) / (64 * waves);
   c.waves = (int)((pieces + 64 * c.chunks - 1) / (64 * c.chunks));
@@ -339,8 +341,10 @@ bool signals_fit(const tfft_scan_args& p) {
 bool signals_fit(const tfft_scan_grad_args& p) {
   return p.share == 1 && p.dy.time == 1 && p.y.time == 1 && p.dx.time == 1 && p.dgate.time == 1 && p.gate.time <= 1;
 }
-Chunking plan_signals(const tfft_scan_args& p) { return plan(p.batch, p.length, p.channels, p.dtype, p.lengths != nullptr); }
-Chunking plan_signals(const tfft_scan_grad_args& p) { return plan(p.batch, p.length, p.channels, p.dtype, p.lengths != nullptr); }
+Chunking plan_signals(const tfft_scan_args& p) { return plan(p.batch, p.length, p.channels, p.dtype, p.lengths != nullptr, kManyRows); }
+Chunking plan_signals(const tfft_scan_grad_args& p) {
+  return plan(p.batch, p.length, p.channels, p.dtype, p.lengths != nullptr, p.dtype == TFFT_F32 ? kManyRows : kManyRowsBack);
+}
 
 void launch_signals(const tfft_scan_args& p, const Chunking& c, word* words, hipStream_t s) {
   const Shape f = shape_of(p, c, words);

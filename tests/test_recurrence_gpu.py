@@ -364,6 +364,12 @@ def test_larger(dim, B, L, D, share):
             assert torch.isfinite(t).all(), name
 
 
+@pytest.mark.parametrize("dim,B,L,D,share", [(1, 1, 66003, 70, 1), (1, 2, 50000, 96, 48), (1, 3, 34000, 40, 1), (2, 20, 17000, 15, 1)])
+def test_long_with_few_channels(dim, B, L, D, share):
+    """The same where groups of chunks are joined in rows of their own, and where a few hundred long signals are taken apart back."""
+    test_larger(dim, B, L, D, share)
+
+
 def test_places():
     """Tensors at one address are taken element for element or refused."""
     x, gate, _, _, _, dy = make(2, 50, 8, states=False)
