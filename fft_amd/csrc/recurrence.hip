@@ -126,7 +126,7 @@ Chunking plan_of(const P& p) {
 }
 unsigned long long parts_of(const tfft_scan_args&) { return 0; }
 unsigned long long parts_of(const tfft_scan_grad_args& p) {
-  return !as_signals(p) && rows_sums_shares(p) ? 4ull * p.batch * p.length * p.channels : 0;
+  return as_signals(p) ? 0 : 4 * rows_parts(p);
 }
 template <class P>
 unsigned long long workspace_of(const P& p) {
@@ -139,8 +139,7 @@ const char* check_plan(const P& p) {
   constexpr long long most = 0xffff0000LL;
   if (p.batch * (p.channels + 3) > kMaxExtent) return large;
   const Chunking c = plan_of(p);
-  if ((__int128)c.blocks() * 64 * c.waves > most) return large;
-  return parts_of(p) && (__int128)p.batch * p.length * (p.channels / p.share) > most ? large : nullptr;
+  return (__int128)c.blocks() * 64 * c.waves > most ? large : nullptr;
 }
 
 // Two tensors at one address: outputs take an input's place element for element, or none at all

@@ -34,7 +34,7 @@ struct Chunking {
   int waves = 0;         // of a workgroup
   int group = 1;         // chunks whose (A, B) are joined directly
   int row = 1;           // groups whose (A, B) are joined directly; the state behind each row of groups is handed on
-  int lanes = 64;        // signals: threads of a row, where a wave holds several rows
+  int lanes = 64;        // rows: lanes that a tile fills; signals: threads of a row, where a wave holds several rows
   bool walks = false;    // a workgroup takes all chunks of its tile, one after the other
   long long state_words = 0;  // states of one chunk
   // 64-bit words: the counters, a map a state and chunk where groups are used and a group where rows of them are, half a word a
@@ -119,7 +119,7 @@ bool rows_vector(const tfft_scan_args& p);
 bool rows_vector(const tfft_scan_grad_args& p);
 Chunking plan_rows(const tfft_scan_args& p);
 Chunking plan_rows(const tfft_scan_grad_args& p);
-bool rows_sums_shares(const tfft_scan_grad_args& p);
+unsigned long long rows_parts(const tfft_scan_grad_args& p);  // fp32 words behind the others, for gates that many channels share
 void launch_rows(const tfft_scan_args& p, const Chunking& c, word* words, hipStream_t s);
 void launch_rows(const tfft_scan_grad_args& p, const Chunking& c, word* words, float* parts, hipStream_t s);
 

@@ -1,5 +1,6 @@
 // The gated linear recurrence where neighbouring channels lie side by side ([batch][time][channel]), and, one element
 // at a time, for any other strides.
+#include <algorithm>
 #include <initializer_list>
 #include <type_traits>
 #include <utility>
@@ -33,17 +34,17 @@ using offset_of = std::conditional_t<V == 1, long long, uint32_t>;
 struct Shape {
   int batch, length, channels, padded;  // padded: channels rounded up to whole runs
   int share, log_gate;
-  int chunks, group, row;
+  int chunks, group, row, lanes;
   long long state_words;
   unsigned tiles_of_entry;  // 0: tiles run through the whole batch
   Turns turns;
   word* words;
 };
 
-// Lane's place: first channel n among the states, batch entry b, first channel c of its run and how many channels of it are the
+// Lane's place: its first word n among those of a chunk's states, batch entry b, first channel c of its run and how many channels of it are the
 // lane's own. The last run of a row that does not fill it lies over the run before, so that every lane can load whole runs:
 // its own channels are the run's last ones, the others' results are dropped. Lanes behind the last channel have none and lie
-// over the tile's first run. first: the batch entry that the tile's addresses start from, the same for all lanes.
+// over the tile's first run. Lanes behind the f.lanes that a tile fills do what the tile's first lanes do, side by side with them. first: the batch entry that the tile's addresses start from, the same for all lanes.
 struct Place {
   unsigned n;
   int b, c, own, first;
@@ -52,13 +53,16 @@ template <int V>
 __device__ __forceinline__ Place place_of(const Shape& f, unsigned tile, int lane) {
   Place p;
   p.n = tile * (64u * V) + lane * V;
+  const unsigned width = f.lanes * V;
+  if (lane >= f.lanes) lane -= f.lanes;
   if (f.tiles_of_entry == 0) {
     p.first = 0;
-    p.b = p.n / (unsigned)f.padded;
-    p.c = p.n - p.b * (unsigned)f.padded;
+    const unsigned m = tile * width + lane * V;
+    p.b = m / (unsigned)f.padded;
+    p.c = m - p.b * (unsigned)f.padded;
   } else {
     p.first = p.b = __builtin_amdgcn_readfirstlane(tile / f.tiles_of_entry);
-    p.c = (tile - p.b * f.tiles_of_entry) * (64 * V) + lane * V;
+    p.c = (tile - p.b * f.tiles_of_entry) * width + lane * V;
   }
   p.own = p.b >= f.batch || p.c >= f.channels ? 0 : min(V, f.channels - p.c);
   if (p.own == 0) p.b = p.first, p.c = 0;
@@ -365,14 +369,19 @@ __device__ __forceinline__ float sum_values(const float (&q)[N], int lane, int l
   }
 }
 
-// Backwards in time: chunk 0 is the latest, wave 0 has the latest piece. `lanes`: lanes that share a gate, 0 where each
-// channel's term goes to `parts` (fp32 [batch][time][channel]) to be summed by a kernel behind.
-template <class T, class G, int V, int VG, bool STREAM>
+// Backwards in time: chunk 0 is the latest, wave 0 has the latest piece. The terms of a gate that several channels share are summed
+// over `lanes` lanes: EVEN by exchanges over a power of two, ODD through LDS, a lane for every gate and step. Where a gate has
+// more lanes than a wave, their sums (ODD) go to `parts` (fp32, [batch][time] and the channels in groups of `lanes` runs) for a
+// kernel behind. B = 8, L = 4096, D = 2048 in bf16 with fp32 gates takes 93 us with 64 channels a gate, D = 2016 with 48 122
+// (1109 with every channel's term in memory), D = 2000 with 200 138 (1048).
+enum { EVEN, ODD };
+template <class T, class G, int V, int VG, bool STREAM, int SUMS = EVEN>
 __global__ __launch_bounds__(64 * kMaxWaves, 4) void scan_rows_bwd(tfft_scan_grad_args p, Shape f, float* parts, int lanes) {
   constexpr int S = kStepsBackward<T>;
   constexpr bool kShared = V == 1 || VG < V;  // a gate may have several channels
   using Off = offset_of<V>;
   __shared__ Joint<V> lds;
+  __shared__ float terms[SUMS == ODD ? kMaxWaves : 1][SUMS == ODD ? S : 1][65];  // 65: lanes read the same place of all steps
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   unsigned tile, chunk;
   if (!take_turn(f.turns, f.words, &lds.ticket, &tile, &chunk)) return;
@@ -439,26 +448,41 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void scan_rows_bwd(tfft_scan_gra
 #pragma unroll
         for (int v = 0; v < V; ++v) q.set(v, da[v]);
         if (in) put<V, STREAM>(dg.here(), q, own);
-      } else if (lanes > 0) {
-        sums[s] = da[0];
+      } else {
+        float sum = da[0];
 #pragma unroll
-        for (int v = 1; v < V; ++v) sums[s] += da[v];
-      } else if (in) {
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-          if (v >= V - own) parts[((long long)at.b * f.length + t) * f.channels + at.c + v] = da[v];
+        for (int v = 1; v < V; ++v) sum += da[v];
+        if constexpr (SUMS == ODD) terms[wave][s][lane] = sum;
+        else sums[s] = sum;
       }
     }
   };
   if (all) walk(std::true_type());
   else walk(std::false_type());
-  if (kShared && f.share > 1) {
+  if constexpr (SUMS == ODD) {
+    // a wave reads what it wrote itself; a barrier would wait for its stores as well
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const int gates = f.lanes / lanes, group = lanes * V;
+    for (int i = lane; i < S * gates; i += 64) {
+      const int s = i / gates, first = (i - s * gates) * lanes, t = t0 + s;
+      float sum = terms[wave][s][first];
+#pragma unroll 4
+      for (int k = 1; k < lanes; ++k) sum += terms[wave][s][first + k];
+      const Place of = place_of<V>(f, tile, first);
+      if (of.own == 0 || t >= f.length) continue;
+      Run<G, 1> q;
+      q.set(0, sum);
+      if (parts) parts[((long long)of.b * f.length + t) * (f.channels / group) + of.c / group] = sum;
+      else store_run<G, 1>(Lane<G, long long>(p.dgate, of, of.c / f.share).at(t), q);
+    }
+  } else if (kShared && f.share > 1) {
     if (lanes >= S) {
       int s = 0;
       Run<G, 1> q;
       q.set(0, sum_values<S>(sums, lane, lanes, s));
       if (at.own > 0 && (lane & (lanes - 1)) < S && t0 + s < f.length) store_run<G, 1>(Lane<G, long long>(p.dgate, at, gate).at(t0 + s), q);
-    } else if (lanes > 0) {
+    } else {
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         for (int m = 1; m < lanes; m *= 2) sums[s] += __shfl_xor(sums[s], m);
@@ -471,16 +495,18 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void scan_rows_bwd(tfft_scan_gra
   if (chunk + 1 == (unsigned)f.chunks && wave == waves - 1) store_state<V>(p.dinitial, at, f.channels, c);
 }
 
-// dgate of a shared gate: its channels' terms summed in their order
+// dgate of a gate that has more lanes than a wave, from the sums of its groups of lanes: 16 threads a gate
 template <class G>
-__global__ __launch_bounds__(256) void sum_shares(tfft_scan_grad_args p, const float* parts) {
-  const long long gates = p.channels / p.share, n = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (n >= p.batch * p.length * gates) return;
-  const long long g = n % gates, bt = n / gates, b = bt / p.length, t = bt % p.length;
-  const float* from = parts + bt * p.channels + g * p.share;
-  float sum = 0.0f;
-  for (long long i = 0; i < p.share; ++i) sum += from[i];
-  ((G*)p.dgate.data)[b * p.dgate.batch + t * p.dgate.time + g * p.dgate.channel] = from_f32<G>(sum);
+__global__ __launch_bounds__(256) void sum_parts(tfft_scan_grad_args p, const float* parts, int groups) {
+  const long long gates = p.channels / p.share, all = p.batch * p.length * gates;
+  const int i = threadIdx.x & 15;
+  for (long long n = 16ll * blockIdx.x + (threadIdx.x >> 4); n < all; n += 16ll * gridDim.x) {
+    float sum = 0.0f;
+    for (int k = i; k < groups; k += 16) sum += parts[n * groups + k];
+    for (int m = 1; m < 16; m *= 2) sum += __shfl_xor(sum, m);
+    const long long g = n % gates, bt = n / gates, b = bt / p.length, t = bt % p.length;
+    if (i == 0) ((G*)p.dgate.data)[b * p.dgate.batch + t * p.dgate.time + g * p.dgate.channel] = from_f32<G>(sum);
+  }
 }
 
 int steps_backward(int dtype) { return dtype == TFFT_F32 ? kStepsBackward<float> : kStepsBackward<f16>; }
@@ -494,16 +520,17 @@ bool through_batch(int run, long long batch, long long channels, std::initialize
   return true;
 }
 
-Chunking plan(long long batch, long long length, long long channels, int run, bool through, int steps, bool padded_batch) {
+Chunking plan(long long batch, long long length, long long channels, int run, int lanes, bool through, int steps, bool padded_batch) {
   Chunking c;
-  const long long padded = (channels + run - 1) / run * run, width = 64 * run;
+  const long long padded = (channels + run - 1) / run * run, width = lanes * run;
+  c.lanes = lanes;
   c.tiles = through ? (batch * padded + width - 1) / width : batch * ((channels + width - 1) / width);
   // as few chunks as the workgroup's waves allow, then as few waves as those need
   const long long pieces = length > 0 ? (length + steps - 1) / steps : 1;
   c.chunks = (pieces + kMaxWaves - 1) / kMaxWaves;
   c.waves = (int)((pieces + c.chunks - 1) / c.chunks);
   c.chunks = (pieces + c.waves - 1) / c.waves;
-  c.state_words = c.tiles * width;
+  c.state_words = c.tiles * 64 * run;
   if (padded_batch && batch > 0) c.strip = c.tiles / (8 * batch) > 1 ? c.tiles / (8 * batch) : 1;
   // About kResident workgroups run at once, kResident / tiles chunks of each tile. That many are joined directly, so that few
   // channels wait for one state in that many chunks, and many channels do not read what they need not: B = 8,
@@ -519,7 +546,7 @@ Chunking plan(long long batch, long long length, long long channels, int run, bo
 template <class P>
 Shape shape_of(const P& p, const Chunking& c, int run, bool through, word* words) {
   return Shape{(int)p.batch, (int)p.length, (int)p.channels, (int)((p.channels + run - 1) / run * run), (int)p.share,
-               p.gate_form == TFFT_GATE_LOG, (int)c.chunks, c.group, c.row, c.state_words, through ? 0u : (unsigned)(c.tiles / p.batch), turns_of(c), words};
+               p.gate_form == TFFT_GATE_LOG, (int)c.chunks, c.group, c.row, c.lanes, c.state_words, through ? 0u : (unsigned)(c.tiles / p.batch), turns_of(c), words};
 }
 
 // Runs of neighbouring channels, all within 32 bits of the row's first one; a gate may be shared by whole runs
@@ -547,21 +574,24 @@ static bool through_batch(const tfft_scan_grad_args& p) {
   return through_batch(run_of_call(p), p.batch, p.channels, {&p.dy, &p.y, &p.gate, &p.dx, &p.dgate});
 }
 Chunking plan_rows(const tfft_scan_args& p) {
-  return plan(p.batch, p.length, p.channels, run_of_call(p), through_batch(p), kStepsForward, p.lengths != nullptr);
+  return plan(p.batch, p.length, p.channels, run_of_call(p), 64, through_batch(p), kStepsForward, p.lengths != nullptr);
+}
+
+// Lanes whose terms a wave sums: all that share a gate, or where those are more than a wave, as large a part of them as divides them. A
+// tile fills as many lanes as such groups do.
+static int lanes_of(const tfft_scan_grad_args& p) {
+  if (p.share == 1) return 1;
+  int lanes = 64;
+  while (p.share / run_of_call(p) % lanes) --lanes;
+  return lanes;
+}
+static int groups_of(const tfft_scan_grad_args& p) { return p.share == 1 ? 1 : (int)(p.share / run_of_call(p) / lanes_of(p)); }
+unsigned long long rows_parts(const tfft_scan_grad_args& p) {
+  return groups_of(p) > 1 ? (unsigned long long)p.batch * p.length * (p.channels / p.share) * groups_of(p) : 0;
 }
 Chunking plan_rows(const tfft_scan_grad_args& p) {
-  return plan(p.batch, p.length, p.channels, run_of_call(p), through_batch(p), steps_backward(p.dtype), p.lengths != nullptr);
+  return plan(p.batch, p.length, p.channels, run_of_call(p), 64 / lanes_of(p) * lanes_of(p), through_batch(p), steps_backward(p.dtype), p.lengths != nullptr);
 }
-
-// Lanes that share a gate, where whole power-of-two groups of a wave's lanes do; 0: summed by a kernel of its own
-static int lanes_of(const tfft_scan_grad_args& p) {
-  const int run = run_of_call(p);
-  if (p.share % run) return 0;
-  const long long lanes = p.share / run;
-  return lanes <= 64 && (lanes & (lanes - 1)) == 0 ? (int)lanes : 0;
-}
-bool rows_sums_shares(const tfft_scan_grad_args& p) { return p.share > 1 && lanes_of(p) == 0; }
-
 // Rows that pass through in whole lines (the gate's too, where every channel has one): B = 8, L = 4096, D = 2048 with fp32 gates
 // takes 107 us forward and 174 back as a stream, 112 and 185 without; D = 2050, where tiles share lines, 140 and 263 against 120
 // and 219.
@@ -593,23 +623,27 @@ void launch_rows(const tfft_scan_args& p, const Chunking& c, word* words, hipStr
 
 void launch_rows(const tfft_scan_grad_args& p, const Chunking& c, word* words, float* parts, hipStream_t s) {
   const bool vector = rows_vector(p);
-  const bool stream = p.channels % kRun == 0 && streams({{&p.dy, p.dtype}, {&p.y, p.dtype}, {&p.dx, p.dtype}}, p.batch, p.length) &&
+  const bool stream = p.channels % kRun == 0 && c.lanes == 64 && streams({{&p.dy, p.dtype}, {&p.y, p.dtype}, {&p.dx, p.dtype}}, p.batch, p.length) &&
                       (p.share > 1 || streams({{&p.gate, p.gate_dtype}, {&p.dgate, p.gate_dtype}}, p.batch, p.length));
   const Shape f = shape_of(p, c, run_of_call(p), through_batch(p), words);
   const dim3 grid((unsigned)c.blocks()), block(64 * c.waves);
-  const int lanes = lanes_of(p);
+  const int lanes = lanes_of(p), groups = groups_of(p);
+  const bool odd = lanes & (lanes - 1) || groups > 1;
+  if (groups == 1) parts = nullptr;
   with_types(p.dtype, p.gate_dtype, [&](auto t, auto g) {
     using T = decltype(t);
     using G = decltype(g);
     constexpr int V = kRun;
-    if (!vector) scan_rows_bwd<T, G, 1, 1, false><<<grid, block, 0, s>>>(p, f, parts, lanes);
+    if (!vector && odd) scan_rows_bwd<T, G, 1, 1, false, ODD><<<grid, block, 0, s>>>(p, f, parts, lanes);
+    else if (!vector) scan_rows_bwd<T, G, 1, 1, false><<<grid, block, 0, s>>>(p, f, parts, lanes);
+    else if (odd) scan_rows_bwd<T, G, V, 1, false, ODD><<<grid, block, 0, s>>>(p, f, parts, lanes);
     else if (p.share == 1 && stream) scan_rows_bwd<T, G, V, V, true><<<grid, block, 0, s>>>(p, f, parts, lanes);
     else if (p.share == 1) scan_rows_bwd<T, G, V, V, false><<<grid, block, 0, s>>>(p, f, parts, lanes);
     else if (stream) scan_rows_bwd<T, G, V, 1, true><<<grid, block, 0, s>>>(p, f, parts, lanes);
     else scan_rows_bwd<T, G, V, 1, false><<<grid, block, 0, s>>>(p, f, parts, lanes);
-    if (rows_sums_shares(p) && p.length > 0) {
+    if (parts && p.length > 0) {
       const long long n = p.batch * p.length * (p.channels / p.share);
-      sum_shares<G><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(p, parts);
+      sum_parts<G><<<(unsigned)std::min((n + 15) / 16, 1LL << 16), 256, 0, s>>>(p, parts, groups);
     }
   });
 }

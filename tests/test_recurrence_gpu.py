@@ -83,6 +83,14 @@ def test_shared_gates(share):
             check_both(*make(B, L, gates * share, share, dtype, gate_dtype, dim, log=k != 1, seed=share + k, ragged=ragged), dim, k != 1)
 
 
+@pytest.mark.parametrize("share", [3, 6, 7, 10, 33, 48, 66, 96, 126, 130, 134, 200, 256])
+@pytest.mark.parametrize("B,L,groups", [(5, 150, 1), (2, 37, 5), (40, 300, 3)])
+def test_shares_that_are_no_power_of_two(share, B, L, groups):
+    """Tiles that leave lanes of a wave empty, in one batch entry and over several, in one chunk and in more."""
+    x, gate, lengths, initial, dlast, dy = make(B, L, groups * share, share, torch.float16, torch.float32, seed=share, ragged=True)
+    check_both(x, gate, lengths, initial, dlast, dy, 1, True)
+
+
 def test_no_states():
     for dim in (1, 2):
         check_both(*make(2, 300, 9, dim=dim, states=False), dim, True)

@@ -77,7 +77,7 @@ def test_null_arguments():
 
 @pytest.mark.parametrize("changes,code", [
     (dict(size=8), INVALID), (dict(dtype=9), UNSUPPORTED), (dict(gate_dtype=F16), UNSUPPORTED), (dict(form=-1), INVALID),
-    (dict(L=9000, workspace=0), INVALID), (dict(share=48, D=96, workspace_bytes=8), INVALID)])
+    (dict(L=9000, workspace=0), INVALID), (dict(share=200, D=400, workspace_bytes=8), INVALID)])
 def test_backward_refusals(changes, code):
     refused(_lib.load().tfft_scan_backward(grad(**changes), None), code)
 
@@ -147,6 +147,7 @@ def test_workspaces():
     assert workspace(scan(B=64, D=768, L=9000, **many)) == (OK, 0)
     rc, need = workspace(scan(B=8, L=4096, D=2048))
     assert rc == OK and 0 < need <= 12 * 8 * 2048 * 32 + 8 * 128
-    rc, need = workspace(backward=grad(B=2, L=100, D=96, share=48))
-    assert rc == OK and need >= 4 * 2 * 100 * 96  # terms of gates whose channels no power of two of lanes holds
+    rc, need = workspace(backward=grad(B=2, L=100, D=400, share=200))
+    assert rc == OK and need == 4 * 2 * 100 * 4  # of gates whose channels a wave does not hold, the sums of halves
+    assert workspace(backward=grad(B=2, L=100, D=96, share=48)) == (OK, 0)
     assert workspace(backward=grad(B=2, L=100, D=64, share=64)) == (OK, 0)
