@@ -91,6 +91,13 @@ def test_shares_that_are_no_power_of_two(share, B, L, groups):
     check_both(x, gate, lengths, initial, dlast, dy, 1, True)
 
 
+@pytest.mark.parametrize("share", [2, 3, 48, 64, 200])
+def test_shared_gates_of_signals(share):
+    """[batch, channel, time] with heads, which goes through the kernels for any strides."""
+    x, gate, lengths, initial, dlast, dy = make(3, 300, 2 * share, share, torch.bfloat16, torch.float32, dim=2, seed=share, ragged=True)
+    check_both(x, gate, lengths, initial, dlast, dy, 2, True)
+
+
 def test_no_states():
     for dim in (1, 2):
         check_both(*make(2, 300, 9, dim=dim, states=False), dim, True)
@@ -287,6 +294,26 @@ def test_streams_and_graphs():
             eager = both(dim, x, g, i, dl, dy)
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(out, eager))
+
+
+def test_two_graphs_at_once():
+    """Two captured calls replayed on two streams at the same time have workspaces of their own."""
+    cases = [make(1, 40000, 128, 1, torch.bfloat16, torch.bfloat16, seed=s) for s in (1, 2)]
+    want = [recurrence.gated_scan(x, g, log_gate=True, initial=i) for x, g, _, i, _, _ in cases]
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in cases], []
+    for graph, (x, g, _, i, _, _) in zip(graphs, cases):
+        with torch.cuda.graph(graph):
+            outs.append(recurrence.gated_scan(x, g, log_gate=True, initial=i))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for stream, graph, out in zip(streams, graphs, outs):
+            with torch.cuda.stream(stream):
+                out[0].zero_()
+                graph.replay()
+        torch.cuda.synchronize()
+        for w, o in zip(want, outs):
+            assert torch.equal(w[0], o[0]) and torch.equal(w[1], o[1])
 
 
 def test_far_offsets():
