@@ -126,7 +126,7 @@ Chunking plan_of(const P& p) {
 }
 unsigned long long parts_of(const tfft_scan_args&) { return 0; }
 unsigned long long parts_of(const tfft_scan_grad_args& p) {
-  return as_signals(p) ? 0 : 4 * rows_parts(p);
+  return 4 * (as_signals(p) ? signals_parts(p) : rows_parts(p));
 }
 template <class P>
 unsigned long long workspace_of(const P& p) {
@@ -226,8 +226,9 @@ extern "C" int tfft_scan_backward(const tfft_scan_grad_args* args, void* stream)
   hipStream_t s = static_cast<hipStream_t>(stream);
   const Chunking c = plan_of(p);
   clear(c, p, s);
-  if (as_signals(p)) launch_signals(p, c, (word*)p.workspace, s);
-  else launch_rows(p, c, (word*)p.workspace, (float*)((word*)p.workspace + c.words()), s);
+  float* parts = (float*)((word*)p.workspace + c.words());
+  if (as_signals(p)) launch_signals(p, c, (word*)p.workspace, parts, s);
+  else launch_rows(p, c, (word*)p.workspace, parts, s);
   return tfft_internal_finish(stream);
 }
 

@@ -128,7 +128,8 @@ bool signals_fit(const tfft_scan_grad_args& p);
 Chunking plan_signals(const tfft_scan_args& p);
 Chunking plan_signals(const tfft_scan_grad_args& p);
 void launch_signals(const tfft_scan_args& p, const Chunking& c, word* words, hipStream_t s);
-void launch_signals(const tfft_scan_grad_args& p, const Chunking& c, word* words, hipStream_t s);
+unsigned long long signals_parts(const tfft_scan_grad_args& p);
+void launch_signals(const tfft_scan_grad_args& p, const Chunking& c, word* words, float* parts, hipStream_t s);
 
 // f(T(), G()) for the element types of a call
 template <class F>

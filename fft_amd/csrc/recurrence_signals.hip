@@ -1,5 +1,8 @@
 // The gated linear recurrence where neighbouring steps lie side by side: the convolution's signals [batch][channel]
-// [time], one gate a channel.
+// [time].
+#include <algorithm>
+#include <type_traits>
+
 #include "recurrence_kernels.hpp"
 
 namespace tfft_seq {
@@ -29,7 +32,7 @@ constexpr int kMaxWaves = 4 * sizeof(T);  // chunks of 8192 steps
 
 struct Shape {
   long long rows;
-  int length, channels, log_gate;
+  int length, channels, share, log_gate;
   int chunks, group, lanes;
   Turns turns;
   word* words;
@@ -199,7 +202,7 @@ __global__ __launch_bounds__(64 * kMaxWaves<T>) void scan_signals_fwd(tfft_scan_
   const int order = threadIdx.x, piece = f.lanes < 64 ? order & (f.lanes - 1) : order;
   const int pieces = f.lanes < 64 ? f.lanes : (int)blockDim.x;
   const T* x = (const T*)p.x.data + b * p.x.batch + c * p.x.channel;
-  const G* g = (const G*)p.gate.data + b * p.gate.batch + c * p.gate.channel;
+  const G* g = (const G*)p.gate.data + b * p.gate.batch + (c / f.share) * p.gate.channel;
   T* y = (T*)p.y.data + b * p.y.batch + c * p.y.channel;
   float start = p.initial ? p.initial[row] : 0.0f, h;
   while (true) {
@@ -234,9 +237,10 @@ __global__ __launch_bounds__(64 * kMaxWaves<T>) void scan_signals_fwd(tfft_scan_
   if (p.last && live && chunk + 1 == (unsigned)f.chunks && piece == pieces - 1) p.last[row] = h;
 }
 
-// Backwards in time: the first thread has the latest steps, chunk 0 is the latest
-template <class T, class G, int MODE>
-__global__ __launch_bounds__(64 * kMaxWaves<T>) void scan_signals_bwd(tfft_scan_grad_args p, Shape f) {
+// Backwards in time: the first thread has the latest steps, chunk 0 is the latest. SHARED: each channel's terms of dgate go to
+// `parts` (fp32, [batch][channel] and rows of `pitch`), to be summed by a kernel behind.
+template <class T, class G, int MODE, bool SHARED>
+__global__ __launch_bounds__(64 * kMaxWaves<T>) void scan_signals_bwd(tfft_scan_grad_args p, Shape f, float* parts, long long pitch) {
   constexpr int E = kSteps<T>;
   __shared__ Lds lds;
   long long row;
@@ -249,7 +253,7 @@ __global__ __launch_bounds__(64 * kMaxWaves<T>) void scan_signals_bwd(tfft_scan_
   const int pieces = f.lanes < 64 ? f.lanes : (int)blockDim.x;
   const T* dy = (const T*)p.dy.data + b * p.dy.batch + c * p.dy.channel;
   const T* y = (const T*)p.y.data + b * p.y.batch + c * p.y.channel;
-  const G* g = (const G*)p.gate.data + b * p.gate.batch + c * p.gate.channel;
+  const G* g = (const G*)p.gate.data + b * p.gate.batch + (c / f.share) * p.gate.channel;
   const float initial = p.initial ? p.initial[row] : 0.0f;
   float start = p.dlast ? p.dlast[row] : 0.0f, k;
   while (true) {
@@ -284,13 +288,17 @@ __global__ __launch_bounds__(64 * kMaxWaves<T>) void scan_signals_bwd(tfft_scan_
       dx[i] = inside ? e : 0.0f;
       k = a[i] * e;
     }
+    using Sum = std::conditional_t<SHARED, float, G>;
     Run<T, E> r;
-    Run<G, E> q;
+    Run<Sum, E> q;
 #pragma unroll
     for (int i = 0; i < E; ++i) r.set(i, dx[i]), q.set(i, dgate[i]);
     if (live) {
       store_steps<E, MODE == SPLIT>((T*)p.dx.data + b * p.dx.batch + c * p.dx.channel, t0, f.length, r);
-      store_steps<E, MODE == SPLIT && sizeof(G) == sizeof(T)>((G*)p.dgate.data + b * p.dgate.batch + c * p.dgate.channel, t0, f.length, q);
+      Sum* to;
+      if constexpr (SHARED) to = parts + row * pitch;
+      else to = (G*)p.dgate.data + b * p.dgate.batch + c * p.dgate.channel;
+      store_steps<E, MODE == SPLIT && sizeof(Sum) == sizeof(T)>(to, t0, f.length, q);
     }
     if (MODE != WALK || chunk + 1 == (unsigned)f.chunks) break;
     start = state_behind(lds, piece == pieces - 1, k);
@@ -298,6 +306,44 @@ __global__ __launch_bounds__(64 * kMaxWaves<T>) void scan_signals_bwd(tfft_scan_
   }
   if (p.dinitial && live && chunk + 1 == (unsigned)f.chunks && piece == pieces - 1) p.dinitial[row] = k;
 }
+
+// dgate of gates that several channels share: 32 threads with kSum steps each side by side, 8 of them for each of those, which take
+// every eighth channel. B = 8, D = 2048, L = 4096 in bf16 with fp32 gates for 64 channels each takes SHAREDUS us back, of which this
+// reads and the kernel before writes 268 MB each; through the kernel for any strides it takes 473.
+constexpr int kSum = 4;
+template <class G>
+__global__ __launch_bounds__(256) void sum_signals(tfft_scan_grad_args p, const float* parts, long long pitch, long long tiles) {
+  __shared__ float lds[8][32][kSum + 1];
+  const int column = threadIdx.x & 31, slice = threadIdx.x >> 5;
+  const long long gates = p.channels / p.share, across = (p.length + 32 * kSum - 1) / (32 * kSum);
+  for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const long long row = tile / across, t = (tile - row * across) * 32 * kSum + column * kSum, b = row / gates, g = row - b * gates;
+    float sum[kSum] = {};
+    if (t < p.length) {  // rows of the parts are whole multiples of kSum
+      const float* from = parts + (row * p.share) * pitch + t;
+#pragma unroll 4
+      for (long long i = slice; i < p.share; i += 8) {
+        const Run<float, kSum> r = load_run<float, kSum>(from + i * pitch);
+#pragma unroll
+        for (int k = 0; k < kSum; ++k) sum[k] += r.get(k);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kSum; ++k) lds[slice][column][k] = sum[k];
+    __syncthreads();
+    if (slice == 0 && t < p.length) {
+      for (int i = 1; i < 8; ++i)
+#pragma unroll
+        for (int k = 0; k < kSum; ++k) sum[k] += lds[i][column][k];
+      Run<G, kSum> q;
+#pragma unroll
+      for (int k = 0; k < kSum; ++k) q.set(k, sum[k]);
+      store_some<kSum>((G*)p.dgate.data + b * p.dgate.batch + g * p.dgate.channel + t, q, (int)min((long long)kSum, p.length - t));
+    }
+    __syncthreads();
+  }
+}
+long long pitch_of(long long length) { return (length + kSum - 1) / kSum * kSum; }
 
 Chunking plan(long long batch, long long length, long long channels, int dtype, bool padded_batch, int many) {
   const int steps = dtype == TFFT_F32 ? kSteps<float> : kSteps<f16>, most = dtype == TFFT_F32 ? kMaxWaves<float> : kMaxWaves<f16>;
@@ -324,7 +370,7 @@ Chunking plan(long long batch, long long length, long long channels, int dtype, 
 
 template <class P>
 Shape shape_of(const P& p, const Chunking& c, word* words) {
-  return Shape{p.batch * p.channels, (int)p.length, (int)p.channels, p.gate_form == TFFT_GATE_LOG,
+  return Shape{p.batch * p.channels, (int)p.length, (int)p.channels, (int)p.share, p.gate_form == TFFT_GATE_LOG,
                (int)c.chunks, c.group, c.lanes, turns_of(c), words};
 }
 
@@ -336,10 +382,10 @@ dim3 grid_of(const Chunking& c) {
 }  // namespace
 
 bool signals_fit(const tfft_scan_args& p) {
-  return p.share == 1 && p.x.time == 1 && p.y.time == 1 && p.gate.time <= 1;
+  return p.x.time == 1 && p.y.time == 1 && p.gate.time <= 1;
 }
 bool signals_fit(const tfft_scan_grad_args& p) {
-  return p.share == 1 && p.dy.time == 1 && p.y.time == 1 && p.dx.time == 1 && p.dgate.time == 1 && p.gate.time <= 1;
+  return p.dy.time == 1 && p.y.time == 1 && p.dx.time == 1 && p.dgate.time == 1 && p.gate.time <= 1;
 }
 Chunking plan_signals(const tfft_scan_args& p) { return plan(p.batch, p.length, p.channels, p.dtype, p.lengths != nullptr, kManyRows); }
 Chunking plan_signals(const tfft_scan_grad_args& p) {
@@ -356,14 +402,23 @@ void launch_signals(const tfft_scan_args& p, const Chunking& c, word* words, hip
     else scan_signals_fwd<T, G, SPLIT><<<grid_of(c), dim3(64 * c.waves), 0, s>>>(p, f);
   });
 }
-void launch_signals(const tfft_scan_grad_args& p, const Chunking& c, word* words, hipStream_t s) {
+unsigned long long signals_parts(const tfft_scan_grad_args& p) { return p.share > 1 ? (unsigned long long)p.batch * p.channels * pitch_of(p.length) : 0; }
+void launch_signals(const tfft_scan_grad_args& p, const Chunking& c, word* words, float* parts, hipStream_t s) {
   const Shape f = shape_of(p, c, words);
+  const long long pitch = pitch_of(p.length);
   with_types(p.dtype, p.gate_dtype, [&](auto t, auto g) {
     using T = decltype(t);
     using G = decltype(g);
-    if (c.chunks <= 1) scan_signals_bwd<T, G, ONE><<<grid_of(c), dim3(64 * c.waves), 0, s>>>(p, f);
-    else if (c.walks) scan_signals_bwd<T, G, WALK><<<grid_of(c), dim3(64 * c.waves), 0, s>>>(p, f);
-    else scan_signals_bwd<T, G, SPLIT><<<grid_of(c), dim3(64 * c.waves), 0, s>>>(p, f);
+    const auto launch = [&](auto shared) {
+      constexpr bool kShared = decltype(shared)::value;
+      if (c.chunks <= 1) scan_signals_bwd<T, G, ONE, kShared><<<grid_of(c), dim3(64 * c.waves), 0, s>>>(p, f, parts, pitch);
+      else if (c.walks) scan_signals_bwd<T, G, WALK, kShared><<<grid_of(c), dim3(64 * c.waves), 0, s>>>(p, f, parts, pitch);
+      else scan_signals_bwd<T, G, SPLIT, kShared><<<grid_of(c), dim3(64 * c.waves), 0, s>>>(p, f, parts, pitch);
+    };
+    if (p.share == 1) return launch(std::false_type());
+    launch(std::true_type());
+    const long long tiles = p.batch * (p.channels / p.share) * ((p.length + 32 * kSum - 1) / (32 * kSum));
+    if (tiles) sum_signals<G><<<(unsigned)std::min(tiles, 1LL << 16), 256, 0, s>>>(p, parts, pitch, tiles);
   });
 }
 

@@ -93,9 +93,14 @@ def test_shares_that_are_no_power_of_two(share, B, L, groups):
 
 @pytest.mark.parametrize("share", [2, 3, 48, 64, 200])
 def test_shared_gates_of_signals(share):
-    """[batch, channel, time] with heads, which goes through the kernels for any strides."""
-    x, gate, lengths, initial, dlast, dy = make(3, 300, 2 * share, share, torch.bfloat16, torch.float32, dim=2, seed=share, ragged=True)
-    check_both(x, gate, lengths, initial, dlast, dy, 2, True)
+    """[batch, channel, time] with heads; lengths of every kind of chunking, and rows that lie apart."""
+    for L in (1, 2, 7, 300, 517, 8193):
+        x, gate, lengths, initial, dlast, dy = make(3, L, 2 * share if L < 1000 else share, share, torch.bfloat16, torch.float32, dim=2, seed=share + L,
+                                                    ragged=True)
+        check_both(x, gate, lengths, initial, dlast, dy, 2, True)
+    x, gate, lengths, initial, dlast, dy = make(2, 203, 3 * share, share, torch.float32, torch.float32, dim=2, log=False)
+    wide = torch.randn(2, 3 * share, 300, device="cuda")
+    check_both(wide[:, :, 5:208], torch.nn.functional.pad(gate, (3, 9))[:, :, 3:206], None, initial, dlast, dy, 2, False)
 
 
 def test_no_states():
@@ -399,7 +404,8 @@ def test_larger(dim, B, L, D, share):
             assert torch.isfinite(t).all(), name
 
 
-@pytest.mark.parametrize("dim,B,L,D,share", [(1, 1, 66003, 70, 1), (1, 2, 50000, 96, 48), (1, 3, 34000, 40, 1), (2, 20, 17000, 15, 1)])
+@pytest.mark.parametrize("dim,B,L,D,share", [(1, 1, 66003, 70, 1), (1, 2, 50000, 96, 48), (1, 3, 34000, 40, 1), (2, 20, 17000, 15, 1),
+                                             (2, 3, 20000, 12, 4), (2, 40, 9000, 30, 10)])
 def test_long_with_few_channels(dim, B, L, D, share):
     """The same where groups of chunks are joined in rows of their own, and where a few hundred long signals are taken apart back."""
     test_larger(dim, B, L, D, share)
