@@ -35,6 +35,7 @@ struct Chunking {
   int group = 1;         // chunks whose (A, B) are joined directly
   int row = 1;           // groups whose (A, B) are joined directly; the state behind each row of groups is handed on
   int lanes = 64;        // rows: lanes that a tile fills; signals: threads of a row, where a wave holds several rows
+  int each = 1;          // signals: rows of a gate that a workgroup takes one after the other
   bool walks = false;    // a workgroup takes all chunks of its tile, one after the other
   long long state_words = 0;  // states of one chunk
   // 64-bit words: the counters, a map a state and chunk where groups are used and a group where rows of them are, half a word a

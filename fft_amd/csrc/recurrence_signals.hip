@@ -24,6 +24,10 @@ constexpr int kMaxGroup = 64;
 // rows on the workgroups have 4 waves, and several of a CU load, wait and store at different times: 49152 x 8200 in bf16 449 us
 // forward and 769 back against 657 and 1351 with 8 waves; with 256 rows they are too few, 96 and 125 us against 65 and 110.
 constexpr int kManyRows = 256, kManyRowsBack = 512, kShortChunks = 1024, kWalkWaves = 4;
+// Rows of a shared gate that a workgroup takes one after the other: up to kEach, or kEachOfFew where that leaves fewer than
+// kFewGroups workgroups. [8, 2048, 4096] in bf16 with 64 channels a gate takes 110, 101, 99, 108 us back with 4, 8, 16, 64 rows (209 with
+// every row's terms in memory), [2, 768, 4096] 19, 22, 33, 103.
+constexpr int kEach = 8, kEachOfFew = 4, kFewGroups = 1024;
 enum { ONE, WALK, SPLIT };  // one chunk, or chunks after one another, or apart
 template <class T>
 constexpr int kSteps = 32 / sizeof(T);
@@ -33,7 +37,7 @@ constexpr int kMaxWaves = 4 * sizeof(T);  // chunks of 8192 steps
 struct Shape {
   long long rows;
   int length, channels, share, log_gate;
-  int chunks, group, lanes;
+  int chunks, group, lanes, each;
   Turns turns;
   word* words;
 };
@@ -307,12 +311,87 @@ __global__ __launch_bounds__(64 * kMaxWaves<T>) void scan_signals_bwd(tfft_scan_
   if (p.dinitial && live && chunk + 1 == (unsigned)f.chunks && piece == pieces - 1) p.dinitial[row] = k;
 }
 
-// dgate of gates that several channels share: 32 threads with kSum steps each side by side, 8 of them for each of those, which take
-// every eighth channel. B = 8, D = 2048, L = 4096 in bf16 with fp32 gates for 64 channels each takes SHAREDUS us back, of which this
-// reads and the kernel before writes 268 MB each; through the kernel for any strides it takes 473.
+// The same for gates that several channels share and rows in one chunk: a workgroup (or a row's lanes) takes f.each rows of a gate
+// one after the other, the next one's loads under way, with the decays and the sums of dgate in registers.
+template <class T, class G>
+__global__ __launch_bounds__(64 * kMaxWaves<T>, 4) void scan_signals_bwd_heads(tfft_scan_grad_args p, Shape f, float* parts, long long pitch) {
+  constexpr int E = kSteps<T>;
+  __shared__ Lds lds[2];  // of this row and the one before: no wave is further apart
+  long long group;
+  unsigned chunk;
+  take<ONE>(f, lds[0], &group, &chunk);
+  const bool live = group < f.rows / f.each;
+  if (!live) group = 0;
+  const unsigned row = (unsigned)group * f.each;
+  const int b = (int)(row / (unsigned)f.channels), c = (int)(row - (unsigned)b * (unsigned)f.channels), len = live ? steps_of(p.lengths, b, f.length) : 0;
+  const int order = threadIdx.x, piece = f.lanes < 64 ? order & (f.lanes - 1) : order;
+  const int pieces = f.lanes < 64 ? f.lanes : (int)blockDim.x, t0 = (pieces - 1 - piece) * E;
+  const T* dy = (const T*)p.dy.data + b * p.dy.batch + c * p.dy.channel;
+  const T* y = (const T*)p.y.data + b * p.y.batch + c * p.y.channel;
+  T* dx = (T*)p.dx.data + b * p.dx.batch + c * p.dx.channel;
+  const G* g = (const G*)p.gate.data + b * p.gate.batch + (c / f.share) * p.gate.channel;
+  const int t_before = min(max(t0 - 1, 0), f.length - 1);
+  Run<G, E> gr = p.gate.time ? ask<E>(g, t0, f.length) : one<E>(g);
+  Run<T, E> d = ask<E>(dy, t0, f.length), own = ask<E>(y, t0, f.length);
+  Run<T, 1> before = load_run<T, 1>(y + t_before);
+  float a[E], sums[E], A = 1.0f;
+  take_decays<E>(gr, p.gate.time, t0, len, f.length, f.log_gate, a);
+#pragma unroll
+  for (int i = E - 1; i >= 0; --i) A *= a[i], sums[i] = 0.0f;
+  for (int n = 0; n < f.each; ++n) {
+    if (n + 1 < f.each) dy += p.dy.channel, y += p.y.channel;
+    const Run<T, E> next_d = ask<E>(dy, t0, f.length), next_own = ask<E>(y, t0, f.length);
+    const Run<T, 1> next_before = load_run<T, 1>(y + t_before);
+    const float initial = p.initial ? p.initial[row + n] : 0.0f;
+    take<E>(d, t0, len, f.length);
+    take<E>(own, t0, len, f.length);
+    float B = 0.0f;
+#pragma unroll
+    for (int i = E - 1; i >= 0; --i) B = a[i] * (B + d.get(i));
+    float k = state_in_front<ONE>(f, lds[n & 1], chunk, row, order, A, B, p.dlast ? p.dlast[row + n] : 0.0f);
+    Run<T, E> r;
+    float e[E];
+#pragma unroll
+    for (int i = E - 1; i >= 0; --i) {
+      e[i] = d.get(i) + k;
+      k = a[i] * e[i];
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const float state = i > 0 ? own.get(i > 0 ? i - 1 : 0) : t0 > 0 ? before.get(0) : initial;
+      const bool inside = t0 + i < len;
+      sums[i] += inside ? e[i] * state : 0.0f;
+      r.set(i, inside ? e[i] : 0.0f);
+    }
+    if (live) store_steps<E, false>(dx, t0, f.length, r);
+    if (p.dinitial && live && piece == pieces - 1) p.dinitial[row + n] = k;
+    dx += p.dx.channel;
+    d = next_d, own = next_own, before = next_before;
+  }
+  if (!live) return;
+  if (f.log_gate) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) sums[i] *= a[i];
+  }
+  if (parts) {
+    Run<float, E> q;
+#pragma unroll
+    for (int i = 0; i < E; ++i) q.set(i, sums[i]);
+    store_steps<E, false>(parts + group * pitch, t0, f.length, q);
+  } else {
+    Run<G, E> q;
+#pragma unroll
+    for (int i = 0; i < E; ++i) q.set(i, sums[i]);
+    store_steps<E, false>((G*)p.dgate.data + b * p.dgate.batch + (c / f.share) * p.dgate.channel, t0, f.length, q);
+  }
+}
+
+// dgate of gates that several channels share, from `count` rows of parts each: 32 threads with kSum steps each side by side, 8 of
+// them for each of those, which take every eighth row. What it reads was written just before, and comes from the last-level cache
+// where it fits.
 constexpr int kSum = 4;
 template <class G>
-__global__ __launch_bounds__(256) void sum_signals(tfft_scan_grad_args p, const float* parts, long long pitch, long long tiles) {
+__global__ __launch_bounds__(256) void sum_signals(tfft_scan_grad_args p, const float* parts, long long pitch, int count, long long tiles) {
   __shared__ float lds[8][32][kSum + 1];
   const int column = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const long long gates = p.channels / p.share, across = (p.length + 32 * kSum - 1) / (32 * kSum);
@@ -320,9 +399,9 @@ __global__ __launch_bounds__(256) void sum_signals(tfft_scan_grad_args p, const 
     const long long row = tile / across, t = (tile - row * across) * 32 * kSum + column * kSum, b = row / gates, g = row - b * gates;
     float sum[kSum] = {};
     if (t < p.length) {  // rows of the parts are whole multiples of kSum
-      const float* from = parts + (row * p.share) * pitch + t;
+      const float* from = parts + row * count * pitch + t;
 #pragma unroll 4
-      for (long long i = slice; i < p.share; i += 8) {
+      for (int i = slice; i < count; i += 8) {
         const Run<float, kSum> r = load_run<float, kSum>(from + i * pitch);
 #pragma unroll
         for (int k = 0; k < kSum; ++k) sum[k] += r.get(k);
@@ -345,7 +424,7 @@ __global__ __launch_bounds__(256) void sum_signals(tfft_scan_grad_args p, const 
 }
 long long pitch_of(long long length) { return (length + kSum - 1) / kSum * kSum; }
 
-Chunking plan(long long batch, long long length, long long channels, int dtype, bool padded_batch, int many) {
+Chunking plan(long long batch, long long length, long long channels, int dtype, bool padded_batch, int many, long long share = 1) {
   const int steps = dtype == TFFT_F32 ? kSteps<float> : kSteps<f16>, most = dtype == TFFT_F32 ? kMaxWaves<float> : kMaxWaves<f16>;
   Chunking c;
   const long long rows = batch * channels, pieces = (length + steps - 1) / steps;
@@ -358,20 +437,26 @@ Chunking plan(long long batch, long long length, long long channels, int dtype, 
     while (c.lanes < pieces) c.lanes *= 2;
     c.waves = 4;
     c.chunks = 1;
-    return c;
+  } else {
+    c.walks = pieces > 64 * most && rows >= many;
+    const int waves = c.walks && rows >= kShortChunks ? kWalkWaves : most;
+    c.chunks = (pieces + 64 * waves - 1) / (64 * waves);
+    c.waves = (int)((pieces + 64 * c.chunks - 1) / (64 * c.chunks));
+    c.chunks = (pieces + 64 * c.waves - 1) / (64 * c.waves);
   }
-  c.walks = pieces > 64 * most && rows >= many;
-  const int waves = c.walks && rows >= kShortChunks ? kWalkWaves : most;
-  c.chunks = (pieces + 64 * waves - 1) / (64 * waves);
-  c.waves = (int)((pieces + 64 * c.chunks - 1) / (64 * c.chunks));
-  c.chunks = (pieces + 64 * c.waves - 1) / (64 * c.waves);
+  if (c.chunks == 1 && length > 0) {
+    const long long groups = c.lanes < 64 ? rows * c.lanes / (64 * c.waves) : rows;
+    c.each = groups >= kEach * kFewGroups ? kEach : kEachOfFew;
+    while (share % c.each) --c.each;
+    c.tiles /= c.each;
+  }
   return c;
 }
 
 template <class P>
 Shape shape_of(const P& p, const Chunking& c, word* words) {
   return Shape{p.batch * p.channels, (int)p.length, (int)p.channels, (int)p.share, p.gate_form == TFFT_GATE_LOG,
-               (int)c.chunks, c.group, c.lanes, turns_of(c), words};
+               (int)c.chunks, c.group, c.lanes, c.each, turns_of(c), words};
 }
 
 dim3 grid_of(const Chunking& c) {
@@ -389,7 +474,7 @@ bool signals_fit(const tfft_scan_grad_args& p) {
 }
 Chunking plan_signals(const tfft_scan_args& p) { return plan(p.batch, p.length, p.channels, p.dtype, p.lengths != nullptr, kManyRows); }
 Chunking plan_signals(const tfft_scan_grad_args& p) {
-  return plan(p.batch, p.length, p.channels, p.dtype, p.lengths != nullptr, p.dtype == TFFT_F32 ? kManyRows : kManyRowsBack);
+  return plan(p.batch, p.length, p.channels, p.dtype, p.lengths != nullptr, p.dtype == TFFT_F32 ? kManyRows : kManyRowsBack, p.share);
 }
 
 void launch_signals(const tfft_scan_args& p, const Chunking& c, word* words, hipStream_t s) {
@@ -402,23 +487,31 @@ void launch_signals(const tfft_scan_args& p, const Chunking& c, word* words, hip
     else scan_signals_fwd<T, G, SPLIT><<<grid_of(c), dim3(64 * c.waves), 0, s>>>(p, f);
   });
 }
-unsigned long long signals_parts(const tfft_scan_grad_args& p) { return p.share > 1 ? (unsigned long long)p.batch * p.channels * pitch_of(p.length) : 0; }
+// Rows of parts a gate; one: none
+static long long parts_of_gate(const tfft_scan_grad_args& p) { return p.length > 0 ? p.share / plan_signals(p).each : 1; }
+unsigned long long signals_parts(const tfft_scan_grad_args& p) {
+  const long long count = parts_of_gate(p);
+  return count > 1 ? (unsigned long long)p.batch * (p.channels / p.share) * count * pitch_of(p.length) : 0;
+}
 void launch_signals(const tfft_scan_grad_args& p, const Chunking& c, word* words, float* parts, hipStream_t s) {
   const Shape f = shape_of(p, c, words);
-  const long long pitch = pitch_of(p.length);
+  const long long pitch = pitch_of(p.length), count = parts_of_gate(p);
+  if (count == 1) parts = nullptr;
   with_types(p.dtype, p.gate_dtype, [&](auto t, auto g) {
     using T = decltype(t);
     using G = decltype(g);
-    const auto launch = [&](auto shared) {
-      constexpr bool kShared = decltype(shared)::value;
-      if (c.chunks <= 1) scan_signals_bwd<T, G, ONE, kShared><<<grid_of(c), dim3(64 * c.waves), 0, s>>>(p, f, parts, pitch);
-      else if (c.walks) scan_signals_bwd<T, G, WALK, kShared><<<grid_of(c), dim3(64 * c.waves), 0, s>>>(p, f, parts, pitch);
-      else scan_signals_bwd<T, G, SPLIT, kShared><<<grid_of(c), dim3(64 * c.waves), 0, s>>>(p, f, parts, pitch);
-    };
-    if (p.share == 1) return launch(std::false_type());
-    launch(std::true_type());
-    const long long tiles = p.batch * (p.channels / p.share) * ((p.length + 32 * kSum - 1) / (32 * kSum));
-    if (tiles) sum_signals<G><<<(unsigned)std::min(tiles, 1LL << 16), 256, 0, s>>>(p, parts, pitch, tiles);
+    const dim3 grid = grid_of(c), block(64 * c.waves);
+    const bool shared = p.share > 1 && p.length > 0;
+    if (c.chunks <= 1 && shared) scan_signals_bwd_heads<T, G><<<grid, block, 0, s>>>(p, f, parts, pitch);
+    else if (c.chunks <= 1) scan_signals_bwd<T, G, ONE, false><<<grid, block, 0, s>>>(p, f, parts, pitch);
+    else if (c.walks && shared) scan_signals_bwd<T, G, WALK, true><<<grid, block, 0, s>>>(p, f, parts, pitch);
+    else if (c.walks) scan_signals_bwd<T, G, WALK, false><<<grid, block, 0, s>>>(p, f, parts, pitch);
+    else if (shared) scan_signals_bwd<T, G, SPLIT, true><<<grid, block, 0, s>>>(p, f, parts, pitch);
+    else scan_signals_bwd<T, G, SPLIT, false><<<grid, block, 0, s>>>(p, f, parts, pitch);
+    if (parts) {
+      const long long tiles = p.batch * (p.channels / p.share) * ((p.length + 32 * kSum - 1) / (32 * kSum));
+      sum_signals<G><<<(unsigned)std::min(tiles, 1LL << 16), 256, 0, s>>>(p, parts, pitch, (int)count, tiles);
+    }
   });
 }
 

@@ -309,8 +309,8 @@ int tfft_get_twiddle_table(int dtype, int n, const void** d_table);
  *
  * Layout: element strides (batch, time, channel; for the gate: batch, time, gate). Any non-negative strides are taken;
  * inputs may repeat (stride 0), outputs may not. Layouts with kernels of their own are channel stride 1 ([batch][time]
- * [channel] activations) and, for share == 1, time stride 1 (the convolution's [batch][channel][time] signals). x and y (dy and
- * dx) may be the same buffer with the same strides; every other overlap of an output with anything gives wrong results.
+ * [channel] activations) and time stride 1 (the convolution's [batch][channel][time] signals). x and y (dy and dx) may
+ * be the same buffer with the same strides; every other overlap of an output with anything gives wrong results.
  *
  * lengths (NULL, or int32 [batch] on the device, clamped to 0 ... length): a padded batch. The steps behind a
  * sequence's length leave its state as it is and do not count (NaN there does no harm); y, dx and dgate are 0 there.

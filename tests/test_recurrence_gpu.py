@@ -101,6 +101,9 @@ def test_shared_gates_of_signals(share):
     x, gate, lengths, initial, dlast, dy = make(2, 203, 3 * share, share, torch.float32, torch.float32, dim=2, log=False)
     wide = torch.randn(2, 3 * share, 300, device="cuda")
     check_both(wide[:, :, 5:208], torch.nn.functional.pad(gate, (3, 9))[:, :, 3:206], None, initial, dlast, dy, 2, False)
+    x, gate, lengths, initial, dlast, dy = make(3, 0, share, share, torch.bfloat16, torch.float32, dim=2)  # no steps: states pass through
+    assert torch.equal(recurrence.gated_scan(x, gate, dim=2, initial=initial)[1], initial)
+    assert torch.equal(recurrence.gated_scan_backward(dy, x, gate, dim=2, initial=initial, dlast=dlast)[2], dlast)
 
 
 def test_no_states():
@@ -405,7 +408,7 @@ def test_larger(dim, B, L, D, share):
 
 
 @pytest.mark.parametrize("dim,B,L,D,share", [(1, 1, 66003, 70, 1), (1, 2, 50000, 96, 48), (1, 3, 34000, 40, 1), (2, 20, 17000, 15, 1),
-                                             (2, 3, 20000, 12, 4), (2, 40, 9000, 30, 10)])
+                                             (2, 3, 20000, 12, 4), (2, 40, 9000, 30, 10), (2, 16, 600, 512, 64)])
 def test_long_with_few_channels(dim, B, L, D, share):
     """The same where groups of chunks are joined in rows of their own, and where a few hundred long signals are taken apart back."""
     test_larger(dim, B, L, D, share)
