@@ -14,7 +14,7 @@ namespace {
 //
 // What bounds it: HBM. B = 64, D = 768, L = 4096 in fp16 takes 200 us forward (1208 MB, 6.0 TB/s) and 340 back (5.9), the same
 // in chunks of 1024, 128 steps; in fp32 32 bytes a thread are 5 % faster than 64 (four accesses to a line, not two). Few long
-// rows do not fill the chip as evenly: 16 signals of 1048573 steps in fp32 back 88 us (335 MB, 3.8 TB/s). Rows at odd addresses
+// rows do not fill the chip as evenly: 16 signals of 1048573 steps in fp32 back 82 us (335 MB, 4.1 TB/s). Rows at odd addresses
 // cost up to a quarter (L = 4095 in bf16 123 us against 103).
 constexpr int kMaxGroup = 64;
 // Longer rows that are many are walked by a workgroup each, chunk after chunk, few rows are split: 256 x 20000 in bf16 takes 11 us
@@ -64,7 +64,7 @@ __device__ __forceinline__ void line_up(Run<T, E>& r, int t0, int length) {
   move_down<E>(r, by);
 }
 // STREAM: as in load_run. Two stores share a line here, which costs a row in one workgroup 1 to 8 %, but where chunks are taken apart the
-// states come through faster: two entries of 8 signals of 1048573 steps in fp32 take 47 us forward and 74 back against 53 and 90.
+// states come through faster: two entries of 8 signals of 1048573 steps in fp32 take 47 us forward and 74 back against 53 and 90 (outputs in the last-level cache).
 template <int E, bool STREAM, class T>
 __device__ __forceinline__ void store_steps(T* p, int t0, int length, const Run<T, E>& r) {
   const int valid = min(max(length - t0, 0), E);
@@ -242,9 +242,13 @@ __global__ __launch_bounds__(64 * kMaxWaves<T>) void scan_signals_fwd(tfft_scan_
 }
 
 // Backwards in time: the first thread has the latest steps, chunk 0 is the latest. SHARED: each channel's terms of dgate go to
-// `parts` (fp32, [batch][channel] and rows of `pitch`), to be summed by a kernel behind.
+// `parts` (fp32, [batch][channel] and rows of `pitch`), to be summed by a kernel behind. kWaves: of a SIMD; chunks taken apart wait
+// for each other, and two workgroups a CU in fp32 (62 registers, where the compiler takes 74) hide that: 16 signals of 1048573 steps
+// 86 -> 82 us, one of 2^24 83 -> 75; 5 waves in 16 bits 294 x 52347 52 -> 49. Whole rows lose 2 %, walked ones spill.
+template <class T, int MODE>
+constexpr int kWaves = MODE != SPLIT ? 1 : sizeof(T) == 4 ? 8 : 5;
 template <class T, class G, int MODE, bool SHARED>
-__global__ __launch_bounds__(64 * kMaxWaves<T>) void scan_signals_bwd(tfft_scan_grad_args p, Shape f, float* parts, long long pitch) {
+__global__ __launch_bounds__(64 * kMaxWaves<T>, (kWaves<T, MODE>)) void scan_signals_bwd(tfft_scan_grad_args p, Shape f, float* parts, long long pitch) {
   constexpr int E = kSteps<T>;
   __shared__ Lds lds;
   long long row;
