@@ -74,26 +74,25 @@ __device__ __forceinline__ Place place_of(const Shape& f, unsigned tile, int lan
 // Vector kernels take 32-bit offsets, so that a load needs no vector register but those that it fills.
 template <class T, class Off>
 struct Lane {
-  char* base;
+  uint64_t base;
   Off off;
   long long step;  // bytes from one time step to the next
   __device__ __forceinline__ Lane(const tfft_seq_view& v, const Place& p, int c)
-      : base((char*)v.data + p.first * v.batch * (long long)sizeof(T)),
+      : base((uint64_t)v.data + p.first * v.batch * (long long)sizeof(T)),
         off((Off)(((p.b - p.first) * v.batch + c * v.channel) * (long long)sizeof(T))),
         step(v.time * (long long)sizeof(T)) {}
   // the lane's address at step t (the same for the wave), and its move to the next or the previous step: an addition in scalar
   // registers, said so for the compiler, which otherwise holds an address a step
   __device__ __forceinline__ void go(int t) {
-    const uint64_t b = (uint64_t)(base + t * step);
-    base = (char*)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32 |
-                   (uint32_t)__builtin_amdgcn_readfirstlane((int)b));
+    const uint64_t b = base + t * step;
+    base = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)b);
   }
   __device__ __forceinline__ void move(long long by) {
     base += by;
     asm("" : "+s"(base));
   }
-  __device__ __forceinline__ T* at(int t) const { return (T*)(base + t * step + off); }
-  __device__ __forceinline__ T* here() const { return (T*)(base + off); }
+  __device__ __forceinline__ T* at(int t) const { return device_pointer<T>(base + t * step, off); }
+  __device__ __forceinline__ T* here() const { return device_pointer<T>(base, off); }
 };
 
 template <int V>

@@ -29,6 +29,14 @@ __device__ __forceinline__ T from_f32(float v) {
 // more than 20, and the scan's vector units are as busy as its memory.
 __device__ __forceinline__ float exp_decay(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
 
+// A pointer to device memory from an address of which the compiler no longer sees where it came from, else it takes the flat
+// loads and stores that could reach LDS too: those wait for LDS and the other way round, and take 64-bit addresses in vector registers.
+template <class T>
+__device__ __forceinline__ T* device_pointer(uint64_t base, uint64_t off = 0) {
+  using Bytes = __attribute__((address_space(1))) char*;
+  return (T*)(char*)((Bytes)base + off);
+}
+
 // N consecutive elements, 16-bit ones two to a register. The copies go through memcpy: the elements' addresses are multiples
 // of the element size only (a row of 770 halves, a slice at an odd offset), and gfx950 loads and stores dwords at any
 // address.
