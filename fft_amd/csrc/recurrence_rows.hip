@@ -333,11 +333,13 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void scan_rows_fwd(tfft_scan_arg
 #pragma unroll
     for (int s = 0; s < S; ++s, y.move(y.step)) {
       Run<T, V> r;
+      float out[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         h[v] = fmaf(a[s][v % VG], h[v], x[s].get(v));
-        r.set(v, whole.value || t0 + s < len ? h[v] : 0.0f);
+        out[v] = whole.value || t0 + s < len ? h[v] : 0.0f;
       }
+      r.set_all(out);
       if (whole.value || t0 + s < f.length) put<V, STREAM>(y.here(), r, whole.value ? V : at.own);
     }
   };
@@ -428,29 +430,31 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void scan_rows_bwd(tfft_scan_gra
     for (int s = S - 1; s >= 0; --s, dx.move(-dx.step), dg.move(-dg.step)) {
       const int t = t0 + s;
       Run<T, V> r;
-      float da[V];
+      float da[V], out[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         const float e = d[s].get(v) + c[v], k = a[s][v % VG];
         float state = before[s].get(v);
         if (s == 0) state = t == 0 ? start[v] : state;
-        r.set(v, whole.value || t < len ? e : 0.0f);
+        out[v] = whole.value || t < len ? e : 0.0f;
         c[v] = k * e;
-        da[v] = (f.log_gate ? c[v] : e) * state;
+        // (a gate's own decay, where it counts, multiplies the sum of its channels)
+        da[v] = VG < V || !f.log_gate ? e * state : c[v] * state;
         if (!whole.value) da[v] = t < len ? da[v] : 0.0f;
       }
+      r.set_all(out);
       const bool in = whole.value || t < f.length;
       const int own = whole.value ? V : at.own;
       if (in) put<V, STREAM>(dx.here(), r, own);
       if (!kShared || (V == 1 && f.share == 1)) {
         Run<G, V> q;
-#pragma unroll
-        for (int v = 0; v < V; ++v) q.set(v, da[v]);
+        q.set_all(da);
         if (in) put<V, STREAM>(dg.here(), q, own);
       } else {
         float sum = da[0];
 #pragma unroll
         for (int v = 1; v < V; ++v) sum += da[v];
+        if (VG < V && f.log_gate) sum *= a[s][0];
         if constexpr (SUMS == ODD) terms[wave][s][lane] = sum;
         else sums[s] = sum;
       }

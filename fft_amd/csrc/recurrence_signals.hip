@@ -228,11 +228,13 @@ __global__ __launch_bounds__(64 * kMaxWaves<T>) void scan_signals_fwd(tfft_scan_
     }
     h = state_in_front<MODE>(f, lds, chunk, row, order, A, B, start);
     Run<T, E> r;
+    float out[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       h = fmaf(a[i], h, xr.get(i));
-      r.set(i, t0 + i < len ? h : 0.0f);
+      out[i] = t0 + i < len ? h : 0.0f;
     }
+    r.set_all(out);
     if (live) store_steps<E, MODE == SPLIT>(y, t0, f.length, r);
     if (MODE != WALK || chunk + 1 == (unsigned)f.chunks) break;
     start = state_behind(lds, piece == pieces - 1, h);
@@ -299,8 +301,7 @@ __global__ __launch_bounds__(64 * kMaxWaves<T>, (kWaves<T, MODE>)) void scan_sig
     using Sum = std::conditional_t<SHARED, float, G>;
     Run<T, E> r;
     Run<Sum, E> q;
-#pragma unroll
-    for (int i = 0; i < E; ++i) r.set(i, dx[i]), q.set(i, dgate[i]);
+    r.set_all(dx), q.set_all(dgate);
     if (live) {
       store_steps<E, MODE == SPLIT>((T*)p.dx.data + b * p.dx.batch + c * p.dx.channel, t0, f.length, r);
       Sum* to;
@@ -365,8 +366,9 @@ __global__ __launch_bounds__(64 * kMaxWaves<T>, 4) void scan_signals_bwd_heads(t
       const float state = i > 0 ? own.get(i > 0 ? i - 1 : 0) : t0 > 0 ? before.get(0) : initial;
       const bool inside = t0 + i < len;
       sums[i] += inside ? e[i] * state : 0.0f;
-      r.set(i, inside ? e[i] : 0.0f);
+      e[i] = inside ? e[i] : 0.0f;
     }
+    r.set_all(e);
     if (live) store_steps<E, false>(dx, t0, f.length, r);
     if (p.dinitial && live && piece == pieces - 1) p.dinitial[row + n] = k;
     dx += p.dx.channel;
@@ -379,13 +381,11 @@ __global__ __launch_bounds__(64 * kMaxWaves<T>, 4) void scan_signals_bwd_heads(t
   }
   if (parts) {
     Run<float, E> q;
-#pragma unroll
-    for (int i = 0; i < E; ++i) q.set(i, sums[i]);
+    q.set_all(sums);
     store_steps<E, false>(parts + group * pitch, t0, f.length, q);
   } else {
     Run<G, E> q;
-#pragma unroll
-    for (int i = 0; i < E; ++i) q.set(i, sums[i]);
+    q.set_all(sums);
     store_steps<E, false>((G*)p.dgate.data + b * p.dgate.batch + (c / f.share) * p.dgate.channel, t0, f.length, q);
   }
 }

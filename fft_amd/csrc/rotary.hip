@@ -104,7 +104,6 @@ __global__ __launch_bounds__(256) void rotary_units(tfft_rotary_args p, Grid g) 
   }
   for (unsigned h0 = hl; h0 < g.heads; h0 += NH * g.lanes) {
     Run<T, R> x[NH], y[NH];
-    T* to[NH];
 #pragma unroll
     for (int j = 0; j < NH; ++j) {
       const unsigned h = h0 + j * g.lanes;
@@ -112,29 +111,35 @@ __global__ __launch_bounds__(256) void rotary_units(tfft_rotary_args p, Grid g) 
         const bool one = h < heads0;
         const long long i = one ? h : h - heads0;
         const T* from = one ? first.in + i * first.in_head : second.in + i * second.in_head;
-        to[j] = (one ? first.out + i * first.out_head : second.out + i * second.out_head) + at;
         x[j] = load_run<T, R>(from + from_x);
         if (HALF && turned) y[j] = load_run<T, R>(from + from_y);
       }
     }
 #pragma unroll
     for (int j = 0; j < NH; ++j) {
-      if (h0 + j * g.lanes >= g.heads) continue;
+      const unsigned h = h0 + j * g.lanes;
+      if (h >= g.heads) continue;
+      const bool one = h < heads0;
+      const long long i = one ? h : h - heads0;
+      T* to = (one ? first.out + i * first.out_head : second.out + i * second.out_head) + at;
       move_down<R>(x[j], at - from_x);
       if (turned) {
         if (HALF) move_down<R>(y[j], at + half - from_y);
-        Run<T, R> re, im;
+        float re[R], im[R];
 #pragma unroll
         for (int k = 0; k < pairs; ++k) {
           const float v = x[j].get(HALF ? k : 2 * k), w = HALF ? y[j].get(k) : x[j].get(HALF ? k : 2 * k + 1);
           const float a = v * c[k] - w * s[k], d = v * s[k] + w * c[k];
-          if (HALF) re.set(k, a), im.set(k, d);
-          else re.set(2 * k, a), re.set(2 * k + 1, d);
+          if (HALF) re[k] = a, im[k] = d;
+          else re[2 * k] = a, re[2 * k + 1] = d;
         }
-        x[j] = re;
-        if (HALF) put<R, STREAM>(to[j] + half, im, valid);
+        x[j].set_all(re);
+        if (HALF) {
+          y[j].set_all(im);
+          put<R, STREAM>(to + half, y[j], valid);
+        }
       }
-      put<R, STREAM>(to[j], x[j], valid);
+      put<R, STREAM>(to, x[j], valid);
     }
   }
 }

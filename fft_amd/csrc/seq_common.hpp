@@ -66,6 +66,23 @@ struct Run {
       else w[i / 2] |= (uint32_t)bits << 16;
     }
   }
+  // elements 2 i and 2 i + 1, in one conversion where the chip has one
+  __device__ __forceinline__ void set_pair(int i, float f0, float f1) {
+    if constexpr (!kHalf) {
+      w[2 * i] = __float_as_uint(f0), w[2 * i + 1] = __float_as_uint(f1);
+    } else {
+      using Two = T __attribute__((ext_vector_type(2)));
+      using Floats = float __attribute__((ext_vector_type(2)));
+      const Two two = __builtin_convertvector((Floats){f0, f1}, Two);
+      __builtin_memcpy(&w[i], &two, 4);
+    }
+  }
+  // all elements
+  __device__ __forceinline__ void set_all(const float (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) set_pair(i, f[2 * i], f[2 * i + 1]);
+    if constexpr (N % 2) set(N - 1, f[N - 1]);
+  }
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (uint32_t& word : w) word = 0;
