@@ -108,12 +108,13 @@ __device__ __forceinline__ void store_state(float* to, const Place& p, int chann
     if (v >= V - p.own) to[(long long)p.b * channels + p.c + v] = h[v];
 }
 
-// The joint map of `count` maps that follow one another, `step` words apart, as soon as they are there
-template <int V>
+// The joint map of `count` maps that follow one another, `step` words apart, as soon as they are there. kAtOnce are read together: 8
+// (65537 x 1024 in bf16 93 us against 96 with 4), or 4 in the kernels for shared gates, which have fewer registers and three workgroups
+// a CU with them ([8, 4096, 2048] with 64 channels a gate 61 us against 67 with 8).
+template <int V, int kAtOnce>
 __device__ __forceinline__ void join_words(const word* from, long long step, int count, float (&a)[V], float (&b)[V]) {
 #pragma unroll
   for (int v = 0; v < V; ++v) a[v] = 1.0f, b[v] = 0.0f;
-  constexpr int kAtOnce = 4;
 #pragma unroll 1
   for (int k = 0; k < count; k += kAtOnce, from += kAtOnce * step) {
     word w[kAtOnce][V];
@@ -137,7 +138,7 @@ __device__ __forceinline__ void join_words(const word* from, long long step, int
 // The state in front of this chunk, for the wave that has the (A, B) of the whole chunk, from the words of earlier chunks (or
 // `start`, in front of the first): the maps of its group's chunks before it, those of the groups before it in their row of
 // groups, and the state in front of that row. Publishes this chunk's own words on the way, each as soon as it is known.
-template <int V>
+template <int V, int kAtOnce>
 __device__ __forceinline__ void state_before(const Shape& f, const float* start, const Place& at, unsigned chunk, const float (&A)[V],
                                              const float (&B)[V], float (&h)[V]) {
   const int r = chunk % f.group, q = chunk / f.group, u = q % f.row, s = q / f.row;
@@ -150,14 +151,14 @@ __device__ __forceinline__ void state_before(const Shape& f, const float* start,
     for (int v = 0; v < V; ++v) publish_map(maps + f.state_words * chunk + v, A[v], B[v]);
   }
   float a[V], b[V];
-  join_words<V>(maps + f.state_words * (chunk - r), f.state_words, r, a, b);
+  join_words<V, kAtOnce>(maps + f.state_words * (chunk - r), f.state_words, r, a, b);
   if (f.row > 1) {
     if (more && last && u != f.row - 1) {
 #pragma unroll
       for (int v = 0; v < V; ++v) publish_map(of_groups + f.state_words * q + v, A[v] * a[v], join(A[v], b[v], B[v]));
     }
     float ga[V], gb[V];
-    join_words<V>(of_groups + f.state_words * (q - u), f.state_words, u, ga, gb);
+    join_words<V, kAtOnce>(of_groups + f.state_words * (q - u), f.state_words, u, ga, gb);
 #pragma unroll
     for (int v = 0; v < V; ++v) b[v] = join(a[v], gb[v], b[v]), a[v] *= ga[v];
   }
@@ -271,7 +272,7 @@ __device__ __forceinline__ void put(T* to, const Run<T, V>& r, int own) {
 }
 
 // From the (A, B) of this wave's piece to the state in front of it
-template <int V>
+template <int V, int kAtOnce>
 __device__ __forceinline__ void state_of_piece(const Shape& f, Joint<V>& lds, const float* start, const Place& at, unsigned chunk, int wave,
                                                int waves, int lane, const float (&A)[V], const float (&B)[V], float (&h)[V]) {
 #pragma unroll
@@ -283,7 +284,7 @@ __device__ __forceinline__ void state_of_piece(const Shape& f, Joint<V>& lds, co
     float chunk_a[V], chunk_b[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) chunk_a[v] = A[v] * front_a[v], chunk_b[v] = join(A[v], front_b[v], B[v]);
-    state_before<V>(f, start, at, chunk, chunk_a, chunk_b, h);
+    state_before<V, kAtOnce>(f, start, at, chunk, chunk_a, chunk_b, h);
 #pragma unroll
     for (int v = 0; v < V; ++v) lds.h[lane * V + v] = h[v];
   }
@@ -325,7 +326,7 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void scan_rows_fwd(tfft_scan_arg
       B[v] = fmaf(a[s][v % VG], B[v], x[s].get(v));
     }
   stay<S, V>(x);
-  state_of_piece<V>(f, lds, p.initial, at, chunk, wave, waves, lane, A, B, h);
+  state_of_piece<V, (VG == V ? 8 : 4)>(f, lds, p.initial, at, chunk, wave, waves, lane, A, B, h);
 
   Lane<T, Off> y(p.y, at, at.c);
   y.go(t0);
@@ -414,7 +415,7 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void scan_rows_bwd(tfft_scan_gra
       B[v] = a[s][v % VG] * (B[v] + d[s].get(v));
     }
   stay<S, V>(d);
-  state_of_piece<V>(f, lds, p.dlast, at, chunk, wave, waves, lane, A, B, c);
+  state_of_piece<V, (VG == V ? 8 : 4)>(f, lds, p.dlast, at, chunk, wave, waves, lane, A, B, c);
 
   take<S, V>(before, t0 - 1, len, all && t0 > 0);
   float start[V];
