@@ -15,17 +15,23 @@ namespace {
 // fill a wave too.
 //
 // What bounds it: HBM, at the rate that this pattern reaches. B = 8, L = 4096, D = 2048 in bf16 with fp32 log decays takes
-// 107 us forward (537 MB, 5.0 TB/s) and 174 back (939 MB, 5.4); as much in chunks that do not depend on each other
-// (B = 64, L = 128, D = 8192) 88 and 158 (6.1, 5.9). The look-back is hidden there (a copy without it takes as long, but
-// for 4 us of clearing its words), with few channels it is not: 65537 x 1024 in bf16 97 us, a copy without it 79.
+// 103 us forward (537 MB, 5.2 TB/s) and 171 back (939 MB, 5.5); as much in chunks that do not depend on each other
+// (B = 64, L = 128, D = 8192) 87 and 156 (6.2, 6.0). The look-back is hidden there but for 4 us of clearing its words; with few
+// channels chunks wait for each other: 65537 x 1024 in bf16 85 us (403 MB, 4.7 TB/s).
 //
-// Why these sizes: 16 steps of two channels are 48 registers of values, which leaves two workgroups of 8 waves a CU that
-// load, wait and store at different times. On those two shapes 24 or 32 steps, runs of 4 and 4, 10, 12 or 16 waves took
-// 0 ... 40 % longer, and a workgroup that takes chunk after chunk with the next one's loads under way 6 %.
+// Why these sizes: 16 steps of two channels are 48 registers of values, 24 in 16 bits 72, which leaves two workgroups of 8 waves a
+// CU that load, wait and store at different times. On those two shapes runs of 4 and 4, 6, 10, 12 or 16 waves took 0 ... 40 %
+// longer, and a workgroup that takes chunk after chunk with the next one's loads under way 6 %.
 constexpr int kMaxWaves = 8, kMaxGroup = 16, kResident = 512, kRun = 2;
-constexpr int kStepsForward = 16;
-template <class T>
-constexpr int kStepsBackward = sizeof(T) == 4 ? 8 : 16;
+// Steps of a piece, forward: kStepsLong of 16-bit values where pieces of kSteps would not fit one chunk, of shared gates (whose kernels
+// have three workgroups a CU with kSteps) from kLongShared steps on. In bf16 with 24 and 16: B = 8, L = 4096, D = 2048 with fp32 log
+// decays 103 and 106 us, one sequence of 65537 x 1024 85 and 94, x 128 20 and 24, [32, 300, 4096] 49 and 52, but [64, 128, 8192]
+// 90 and 87; 64 channels a gate: 65537 x 1024 70 and 78, [16, 500, 1024] 14 and 13. In fp32 [4, 3000, 600] 27.5 and 25.
+constexpr int kSteps = 16, kStepsLong = 24, kLongShared = 4096;
+// Backward: where a run of channels has one gate, fewer decays leave registers for more steps: 4 entries of up to 8191 steps with heads of
+// 64 in bf16 83 us against 87 with 16, [8, 4096, 2048] in fp32 145 against 154 with 8. With a gate a channel 20 take 175 us where 16 take 171.
+template <class T, bool kOneGate>
+constexpr int kStepsBackward = sizeof(T) == 4 ? (kOneGate ? 12 : 8) : kOneGate ? 20 : 16;
 
 // Runs take 32-bit offsets, which the plan has checked; single elements may lie anywhere
 template <int V>
@@ -108,13 +114,12 @@ __device__ __forceinline__ void store_state(float* to, const Place& p, int chann
     if (v >= V - p.own) to[(long long)p.b * channels + p.c + v] = h[v];
 }
 
-// The joint map of `count` maps that follow one another, `step` words apart, as soon as they are there. kAtOnce are read together: 8
-// (65537 x 1024 in bf16 93 us against 96 with 4), or 4 in the kernels for shared gates, which have fewer registers and three workgroups
-// a CU with them ([8, 4096, 2048] with 64 channels a gate 61 us against 67 with 8).
-template <int V, int kAtOnce>
+// The joint map of `count` maps that follow one another, `step` words apart, as soon as they are there
+template <int V>
 __device__ __forceinline__ void join_words(const word* from, long long step, int count, float (&a)[V], float (&b)[V]) {
 #pragma unroll
   for (int v = 0; v < V; ++v) a[v] = 1.0f, b[v] = 0.0f;
+  constexpr int kAtOnce = 4;
 #pragma unroll 1
   for (int k = 0; k < count; k += kAtOnce, from += kAtOnce * step) {
     word w[kAtOnce][V];
@@ -138,7 +143,7 @@ __device__ __forceinline__ void join_words(const word* from, long long step, int
 // The state in front of this chunk, for the wave that has the (A, B) of the whole chunk, from the words of earlier chunks (or
 // `start`, in front of the first): the maps of its group's chunks before it, those of the groups before it in their row of
 // groups, and the state in front of that row. Publishes this chunk's own words on the way, each as soon as it is known.
-template <int V, int kAtOnce>
+template <int V>
 __device__ __forceinline__ void state_before(const Shape& f, const float* start, const Place& at, unsigned chunk, const float (&A)[V],
                                              const float (&B)[V], float (&h)[V]) {
   const int r = chunk % f.group, q = chunk / f.group, u = q % f.row, s = q / f.row;
@@ -151,14 +156,14 @@ __device__ __forceinline__ void state_before(const Shape& f, const float* start,
     for (int v = 0; v < V; ++v) publish_map(maps + f.state_words * chunk + v, A[v], B[v]);
   }
   float a[V], b[V];
-  join_words<V, kAtOnce>(maps + f.state_words * (chunk - r), f.state_words, r, a, b);
+  join_words<V>(maps + f.state_words * (chunk - r), f.state_words, r, a, b);
   if (f.row > 1) {
     if (more && last && u != f.row - 1) {
 #pragma unroll
       for (int v = 0; v < V; ++v) publish_map(of_groups + f.state_words * q + v, A[v] * a[v], join(A[v], b[v], B[v]));
     }
     float ga[V], gb[V];
-    join_words<V, kAtOnce>(of_groups + f.state_words * (q - u), f.state_words, u, ga, gb);
+    join_words<V>(of_groups + f.state_words * (q - u), f.state_words, u, ga, gb);
 #pragma unroll
     for (int v = 0; v < V; ++v) b[v] = join(a[v], gb[v], b[v]), a[v] *= ga[v];
   }
@@ -272,7 +277,7 @@ __device__ __forceinline__ void put(T* to, const Run<T, V>& r, int own) {
 }
 
 // From the (A, B) of this wave's piece to the state in front of it
-template <int V, int kAtOnce>
+template <int V>
 __device__ __forceinline__ void state_of_piece(const Shape& f, Joint<V>& lds, const float* start, const Place& at, unsigned chunk, int wave,
                                                int waves, int lane, const float (&A)[V], const float (&B)[V], float (&h)[V]) {
 #pragma unroll
@@ -284,7 +289,7 @@ __device__ __forceinline__ void state_of_piece(const Shape& f, Joint<V>& lds, co
     float chunk_a[V], chunk_b[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) chunk_a[v] = A[v] * front_a[v], chunk_b[v] = join(A[v], front_b[v], B[v]);
-    state_before<V, kAtOnce>(f, start, at, chunk, chunk_a, chunk_b, h);
+    state_before<V>(f, start, at, chunk, chunk_a, chunk_b, h);
 #pragma unroll
     for (int v = 0; v < V; ++v) lds.h[lane * V + v] = h[v];
   }
@@ -293,9 +298,8 @@ __device__ __forceinline__ void state_of_piece(const Shape& f, Joint<V>& lds, co
   for (int v = 0; v < V; ++v) h[v] = join(front_a[v], lds.h[lane * V + v], front_b[v]);
 }
 
-template <class T, class G, int V, int VG, bool STREAM>
+template <class T, class G, int V, int VG, bool STREAM, int S>
 __global__ __launch_bounds__(64 * kMaxWaves, 4) void scan_rows_fwd(tfft_scan_args p, Shape f) {
-  constexpr int S = kStepsForward;
   using Off = offset_of<V>;
   __shared__ Joint<V> lds;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
@@ -326,7 +330,7 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void scan_rows_fwd(tfft_scan_arg
       B[v] = fmaf(a[s][v % VG], B[v], x[s].get(v));
     }
   stay<S, V>(x);
-  state_of_piece<V, (VG == V ? 8 : 4)>(f, lds, p.initial, at, chunk, wave, waves, lane, A, B, h);
+  state_of_piece<V>(f, lds, p.initial, at, chunk, wave, waves, lane, A, B, h);
 
   Lane<T, Off> y(p.y, at, at.c);
   y.go(t0);
@@ -374,12 +378,12 @@ __device__ __forceinline__ float sum_values(const float (&q)[N], int lane, int l
 // Backwards in time: chunk 0 is the latest, wave 0 has the latest piece. The terms of a gate that several channels share are summed
 // over `lanes` lanes: EVEN by exchanges over a power of two, ODD through LDS, a lane for every gate and step. Where a gate has
 // more lanes than a wave, their sums (ODD) go to `parts` (fp32, [batch][time] and the channels in groups of `lanes` runs) for a
-// kernel behind. B = 8, L = 4096, D = 2048 in bf16 with fp32 gates takes 93 us with 64 channels a gate, D = 2016 with 48 122
-// (1109 with every channel's term in memory), D = 2000 with 200 138 (1048).
+// kernel behind. B = 8, L = 4096, D = 2048 in bf16 with fp32 gates takes 85 us with 64 channels a gate, D = 2016 with 48 110
+// (1109 with every channel's term in memory), D = 2000 with 200 128 (1048).
 enum { EVEN, ODD };
 template <class T, class G, int V, int VG, bool STREAM, int SUMS = EVEN>
 __global__ __launch_bounds__(64 * kMaxWaves, 4) void scan_rows_bwd(tfft_scan_grad_args p, Shape f, float* parts, int lanes) {
-  constexpr int S = kStepsBackward<T>;
+  constexpr int S = kStepsBackward<T, (VG < V)>;
   constexpr bool kShared = V == 1 || VG < V;  // a gate may have several channels
   using Off = offset_of<V>;
   __shared__ Joint<V> lds;
@@ -415,7 +419,7 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void scan_rows_bwd(tfft_scan_gra
       B[v] = a[s][v % VG] * (B[v] + d[s].get(v));
     }
   stay<S, V>(d);
-  state_of_piece<V, (VG == V ? 8 : 4)>(f, lds, p.dlast, at, chunk, wave, waves, lane, A, B, c);
+  state_of_piece<V>(f, lds, p.dlast, at, chunk, wave, waves, lane, A, B, c);
 
   take<S, V>(before, t0 - 1, len, all && t0 > 0);
   float start[V];
@@ -481,11 +485,26 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void scan_rows_bwd(tfft_scan_gra
       else store_run<G, 1>(Lane<G, long long>(p.dgate, of, of.c / f.share).at(t), q);
     }
   } else if (kShared && f.share > 1) {
-    if (lanes >= S) {
-      int s = 0;
-      Run<G, 1> q;
-      q.set(0, sum_values<S>(sums, lane, lanes, s));
-      if (at.own > 0 && (lane & (lanes - 1)) < S && t0 + s < f.length) store_run<G, 1>(Lane<G, long long>(p.dgate, at, gate).at(t0 + s), q);
+    constexpr int kFirst = S >= 16 ? 16 : 8, kRest = S - kFirst;  // powers of two
+    if (lanes >= kFirst) {
+      const auto give = [&](const auto& some, auto count, int first) {
+        constexpr int kCount = decltype(count)::value;
+        int s = 0;
+        Run<G, 1> q;
+        q.set(0, sum_values<kCount>(some, lane, lanes, s));
+        s += first;
+        if (at.own > 0 && (lane & (lanes - 1)) < kCount && t0 + s < f.length) store_run<G, 1>(Lane<G, long long>(p.dgate, at, gate).at(t0 + s), q);
+      };
+      float some[kFirst];
+#pragma unroll
+      for (int i = 0; i < kFirst; ++i) some[i] = sums[i];
+      give(some, std::integral_constant<int, kFirst>(), 0);
+      if constexpr (kRest > 0) {
+        float rest[kRest];
+#pragma unroll
+        for (int i = 0; i < kRest; ++i) rest[i] = sums[kFirst + i];
+        give(rest, std::integral_constant<int, kRest>(), kFirst);
+      }
     } else {
 #pragma unroll
       for (int s = 0; s < S; ++s) {
@@ -513,7 +532,10 @@ __global__ __launch_bounds__(256) void sum_parts(tfft_scan_grad_args p, const fl
   }
 }
 
-int steps_backward(int dtype) { return dtype == TFFT_F32 ? kStepsBackward<float> : kStepsBackward<f16>; }
+int steps_backward(int dtype, bool one_gate) {
+  if (one_gate) return dtype == TFFT_F32 ? kStepsBackward<float, true> : kStepsBackward<f16, true>;
+  return dtype == TFFT_F32 ? kStepsBackward<float, false> : kStepsBackward<f16, false>;
+}
 
 // Tiles run through the whole batch where that keeps a lane's offsets within 32 bits, so that few channels fill a wave too; else
 // each batch entry has tiles of its own.
@@ -577,8 +599,11 @@ static bool through_batch(const tfft_scan_args& p) {
 static bool through_batch(const tfft_scan_grad_args& p) {
   return through_batch(run_of_call(p), p.batch, p.channels, {&p.dy, &p.y, &p.gate, &p.dx, &p.dgate});
 }
+static bool long_pieces(const tfft_scan_args& p) {
+  return p.dtype != TFFT_F32 && rows_vector(p) && (p.share == 1 ? p.length > kMaxWaves * kSteps : p.length >= kLongShared);
+}
 Chunking plan_rows(const tfft_scan_args& p) {
-  return plan(p.batch, p.length, p.channels, run_of_call(p), 64, through_batch(p), kStepsForward, p.lengths != nullptr);
+  return plan(p.batch, p.length, p.channels, run_of_call(p), 64, through_batch(p), long_pieces(p) ? kStepsLong : kSteps, p.lengths != nullptr);
 }
 
 // Lanes whose terms a wave sums: all that share a gate, or where those are more than a wave, as large a part of them as divides them. A
@@ -594,7 +619,7 @@ unsigned long long rows_parts(const tfft_scan_grad_args& p) {
   return groups_of(p) > 1 ? (unsigned long long)p.batch * p.length * (p.channels / p.share) * groups_of(p) : 0;
 }
 Chunking plan_rows(const tfft_scan_grad_args& p) {
-  return plan(p.batch, p.length, p.channels, run_of_call(p), 64 / lanes_of(p) * lanes_of(p), through_batch(p), steps_backward(p.dtype), p.lengths != nullptr);
+  return plan(p.batch, p.length, p.channels, run_of_call(p), 64 / lanes_of(p) * lanes_of(p), through_batch(p), steps_backward(p.dtype, rows_vector(p) && p.share > 1), p.lengths != nullptr);
 }
 // Rows that pass through in whole lines (the gate's too, where every channel has one): B = 8, L = 4096, D = 2048 with fp32 gates
 // takes 107 us forward and 174 back as a stream, 112 and 185 without; D = 2050, where tiles share lines, 140 and 263 against 120
@@ -617,11 +642,17 @@ void launch_rows(const tfft_scan_args& p, const Chunking& c, word* words, hipStr
     using T = decltype(t);
     using G = decltype(g);
     constexpr int V = kRun;
-    if (!vector) scan_rows_fwd<T, G, 1, 1, false><<<grid, block, 0, s>>>(p, f);
-    else if (p.share == 1 && stream) scan_rows_fwd<T, G, V, V, true><<<grid, block, 0, s>>>(p, f);
-    else if (p.share == 1) scan_rows_fwd<T, G, V, V, false><<<grid, block, 0, s>>>(p, f);
-    else if (stream) scan_rows_fwd<T, G, V, 1, true><<<grid, block, 0, s>>>(p, f);
-    else scan_rows_fwd<T, G, V, 1, false><<<grid, block, 0, s>>>(p, f);
+    const auto launch = [&](auto steps) {
+      constexpr int S = decltype(steps)::value;
+      if (p.share == 1 && stream) scan_rows_fwd<T, G, V, V, true, S><<<grid, block, 0, s>>>(p, f);
+      else if (p.share == 1) scan_rows_fwd<T, G, V, V, false, S><<<grid, block, 0, s>>>(p, f);
+      else if (stream) scan_rows_fwd<T, G, V, 1, true, S><<<grid, block, 0, s>>>(p, f);
+      else scan_rows_fwd<T, G, V, 1, false, S><<<grid, block, 0, s>>>(p, f);
+    };
+    if (!vector) return scan_rows_fwd<T, G, 1, 1, false, kSteps><<<grid, block, 0, s>>>(p, f);
+    if constexpr (sizeof(T) == 2)
+      if (long_pieces(p)) return launch(std::integral_constant<int, kStepsLong>());
+    launch(std::integral_constant<int, kSteps>());
   });
 }
 
