@@ -14,11 +14,11 @@
 // ends. The order of all sums is fixed by the sizes.
 //
 // Each of the eight XCDs has a counter of its own, with all chunks of an eighth of the tiles, neighbours beside each other (workgroups
-// go round the XCDs): an XCD then reads whole rows, and lines that two tiles share once. B = 8, L = 4096 with D = 2048: 112 us forward
-// and 184 back, where the XCDs take every eighth tile 116 and 195; with D = 2050 120 and 219 against 140 and 251. With fewer than
-// kManyTiles tiles an eighth is too narrow, and all take from one counter, chunk by chunk: 65537 x 1152 (9 tiles) 129 us against
-// 197 with eight. In a padded batch an XCD has a strip of every entry instead, or the one with the longest sequences would be
-// the last to end (4 entries of up to 8191 steps, heads of 64: 94 us against 97 back).
+// go round the XCDs): an XCD then reads whole rows, and lines that two tiles share once. B = 8, L = 4096 with D = 2048: 103 us forward
+// and 170 back, where the XCDs take every eighth tile 106 and 182; with D = 2050 125 and 222 against 142 and 258. With fewer than
+// kManyTiles tiles an eighth is too narrow, and all take from one counter, chunk by chunk: 65537 x 1152 (9 tiles) 93 us against
+// 134 with eight. In a padded batch an XCD has a strip of every entry instead, or the one with the longest sequences would be
+// the last to end: 8 entries of 1024 channels, one of 16384 steps and seven of 1000, 114 us forward and 204 back against 170 and 291.
 #pragma once
 #include "seq_common.hpp"
 

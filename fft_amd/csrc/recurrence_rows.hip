@@ -47,10 +47,11 @@ struct Shape {
   word* words;
 };
 
-// Lane's place: its first word n among those of a chunk's states, batch entry b, first channel c of its run and how many channels of it are the
-// lane's own. The last run of a row that does not fill it lies over the run before, so that every lane can load whole runs:
-// its own channels are the run's last ones, the others' results are dropped. Lanes behind the last channel have none and lie
-// over the tile's first run. Lanes behind the f.lanes that a tile fills do what the tile's first lanes do, side by side with them. first: the batch entry that the tile's addresses start from, the same for all lanes.
+// Lane's place: its first word n among those of a chunk's states, batch entry b, first channel c of its run and how many
+// channels of it are the lane's own. The last run of a row that does not fill it lies over the run before, so that every lane can
+// load whole runs: its own channels are the run's last ones, the others' results are dropped. Lanes behind the last channel have
+// none and lie over the tile's first run. Lanes behind the f.lanes that a tile fills do what the tile's first lanes do, side by
+// side with them. first: the batch entry that the tile's addresses start from, the same for all lanes.
 struct Place {
   unsigned n;
   int b, c, own, first;
@@ -560,11 +561,11 @@ Chunking plan(long long batch, long long length, long long channels, int run, in
   if (padded_batch && batch > 0) c.strip = c.tiles / (8 * batch) > 1 ? c.tiles / (8 * batch) : 1;
   // About kResident workgroups run at once, kResident / tiles chunks of each tile. That many are joined directly, so that few
   // channels wait for one state in that many chunks, and many channels do not read what they need not: B = 8,
-  // L = 4096, D = 2048 (128 tiles) takes 118, 121, 129 us with groups of 4, 8, 16; one sequence of 65537 steps
-  // and 1024 channels (8 tiles) 180, 129, 119 us.
+  // L = 4096, D = 2048 (128 tiles) takes 170, 170, 172 us back with groups of 4, 8, 16; one sequence of 65537 steps
+  // and 1024 channels (8 tiles) 101, 86, 85 us forward.
   while (c.group < kMaxGroup && c.group * c.tiles < kResident) c.group *= 2;
   // With one or two tiles the states of one group after the other are what a call waits for: one sequence of 65537 steps in bf16 takes
-  // 39, 46 us with 128, 256 channels so, 24, 36 in rows of groups; with 1024 channels 96 against 102.
+  // 30, 39 us with 128, 256 channels so, 20, 35 in rows of groups; with 1024 channels rows of groups cost 6 %.
   if (c.tiles <= 2) c.row = kMaxGroup;
   return c;
 }
@@ -622,8 +623,8 @@ Chunking plan_rows(const tfft_scan_grad_args& p) {
   return plan(p.batch, p.length, p.channels, run_of_call(p), 64 / lanes_of(p) * lanes_of(p), through_batch(p), steps_backward(p.dtype, rows_vector(p) && p.share > 1), p.lengths != nullptr);
 }
 // Rows that pass through in whole lines (the gate's too, where every channel has one): B = 8, L = 4096, D = 2048 with fp32 gates
-// takes 107 us forward and 174 back as a stream, 112 and 185 without; D = 2050, where tiles share lines, 140 and 263 against 120
-// and 219.
+// takes 103 us forward and 170 back as a stream, 111 and 183 without; D = 2050, where tiles share lines, 142 and 265 against 125
+// and 222.
 static bool streams(std::initializer_list<std::pair<const tfft_seq_view*, int>> views, long long batch, long long length) {
   for (const auto& [v, dtype] : views) {
     const long long stride[2] = {v->batch, v->time}, extent[2] = {batch, length};
