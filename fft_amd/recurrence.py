@@ -28,7 +28,7 @@ def _placed(call, device, stream, *args):
     """call(*args, raw stream) with torch's current device and stream those of the call, so that what it allocates belongs to
     the stream that it runs on. device: an index. Switching costs more than a short kernel, so it is left out where nothing
     changes."""
-    if stream is None and device == torch.cuda.current_device():
+    if stream is None and device == torch._C._cuda_getDevice():
         return call(*args, torch._C._cuda_getCurrentRawStream(device))
     if stream is not None and stream.device.index != device:
         _refuse(f"{call.__name__.lstrip('_')}: the stream belongs to {stream.device}, the tensors to cuda:{device}")
@@ -57,6 +57,12 @@ def _same_device(who, x, *others):
         if t is not None and t.get_device() != device:
             _refuse(f"{who}: tensors on {x.device} and {t.device}")
     return device
+
+
+def _values(*tensors):
+    """The tensors with their values in memory: torch only notes some negations (the imaginary part of a conjugated tensor),
+    and what lies at their address has the other sign. Runs on the call's stream."""
+    return [t if t is None else t.resolve_neg() for t in tensors]
 
 
 def _state(who, name, t, B, D):
@@ -96,8 +102,8 @@ def _sizes(who, x, gate, dim):
 def _out(who, name, t, like):
     if t is None:
         return torch.empty_like(like, memory_format=torch.contiguous_format)
-    if t.dtype != like.dtype or t.shape != like.shape:
-        _refuse(f"{who}: {name} is a {like.dtype} tensor {tuple(like.shape)}")
+    if t.dtype != like.dtype or t.shape != like.shape or t.is_neg():
+        _refuse(f"{who}: {name} is a {like.dtype} tensor {tuple(like.shape)}, no negated view")
     return t
 
 
@@ -124,13 +130,16 @@ def gated_scan(x, gate, dim=1, log_gate=False, lengths=None, initial=None, out=N
     x: [B, L, D] (dim = 1) or [B, D, L] (dim = 2), float32, float16 or bfloat16, any strides. gate: the same with G
     channels, one for D / G neighbours, of x's type or float32; with log_gate the decay is exp(gate). lengths (int32
     [B]): steps behind a sequence's length do not count, leave the state as it is, and y is 0 there. initial: fp32
-    [B, D]. out: a tensor for y, x itself allowed. Asynchronous on `stream` (default: torch's current stream)."""
+    [B, D]. out: a tensor for y, x itself allowed. Inputs count by their values, a negation that torch has only noted
+    (z.conj().imag) included; into such a view nothing is written. Asynchronous on `stream` (default: torch's current stream)."""
     return _placed(_gated_scan, _same_device("gated_scan", x, gate, lengths, initial, out), stream, x, gate, dim, log_gate,
                    lengths, initial, out)
 
 
 def _gated_scan(x, gate, dim, log_gate, lengths, initial, out, stream):
     who = "gated_scan"
+    if any(t is not None and t.is_neg() for t in (x, gate, lengths, initial)):
+        x, gate, lengths, initial = _values(x, gate, lengths, initial)
     code, gate_code = _types(who, x, gate)
     B, L, D, share = _sizes(who, x, gate, dim)
     y = _out(who, "out", out, x)
@@ -156,6 +165,8 @@ def gated_scan_backward(dy, y, gate, dim=1, log_gate=False, lengths=None, initia
 
 def _gated_scan_backward(dy, y, gate, dim, log_gate, lengths, initial, dlast, dx, dgate, stream):
     who = "gated_scan_backward"
+    if any(t is not None and t.is_neg() for t in (dy, y, gate, lengths, initial, dlast)):
+        dy, y, gate, lengths, initial, dlast = _values(dy, y, gate, lengths, initial, dlast)
     code, gate_code = _types(who, dy, gate)
     B, L, D, share = _sizes(who, dy, gate, dim)
     if y.dtype != dy.dtype or y.shape != dy.shape:
@@ -189,6 +200,10 @@ def _gated_scan_step(x, gate, state, log_gate, new_state, out, stream):
         _refuse(f"{who}: {G} gates do not divide {D} channels")
     if new_state is None:
         new_state = state
+    if new_state.is_neg():
+        _refuse(f"{who}: a state that is written into is no negated view")
+    if x.is_neg() or gate.is_neg() or (state is not new_state and state.is_neg()):
+        x, gate, state = _values(x, gate, state)
     for t in (state,) if new_state is state else (state, new_state):
         if t.dtype != torch.float32 or t.shape != shape:
             _refuse(f"{who}: state and new_state are float32 tensors [{B}, {D}]")

@@ -15,7 +15,7 @@ import torch
 
 from . import _lib
 from .api import _check
-from .recurrence import _FLOATS, _placed, _refuse, _same_device
+from .recurrence import _FLOATS, _placed, _refuse, _same_device, _values
 
 _PAIRS = {"half": 0, "interleaved": 1}
 _POSITIONS = {torch.int64: 8, torch.int32: 4}
@@ -78,7 +78,7 @@ def rotate(plan, q, k=None, positions=None, pairs="half", inverse=False, first=0
     plan.size of the P values are rotated, the rest copied. pairs: "half" pairs value i with i + size / 2, "interleaved"
     2 i with 2 i + 1. positions: int64 or int32 [B, L] or [L] on the device (negative ones turn backwards); without
     them position t is first + t. inverse: the other way round, which is the gradient of rotate. out, out_k: tensors for the results,
-    q and k themselves allowed. Asynchronous on `stream` (default: torch's current stream)."""
+    q and k themselves allowed (but no view that torch has only noted as negated). Asynchronous on `stream` (default: torch's current stream)."""
     device = _same_device("rotate", q, k, plan.turns, positions, out, out_k)
     return _placed(_rotate, device, stream, plan, q, k, positions, pairs, inverse, first, out, out_k)
 
@@ -88,6 +88,8 @@ _NO_TENSOR = (0,) * 9
 
 def _rotate(plan, q, k, positions, pairs, inverse, first, out, out_k, stream):
     who = "rotate"
+    if q.is_neg() or (k is not None and k.is_neg()) or (positions is not None and positions.is_neg()):
+        q, k, positions = _values(q, k, positions)
     dtype, shape = q.dtype, q.shape
     code = _FLOATS.get(dtype)
     if code is None:
@@ -113,8 +115,8 @@ def _rotate(plan, q, k, positions, pairs, inverse, first, out, out_k, stream):
         at = positions.data_ptr()
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif out.dtype != dtype or out.shape != shape:
-        _refuse(f"{who}: the result of q is a {dtype} tensor {tuple(shape)}")
+    elif out.dtype != dtype or out.shape != shape or out.is_neg():
+        _refuse(f"{who}: the result of q is a {dtype} tensor {tuple(shape)}, no negated view")
     first_view = _view(who, q, out, H, P)
     if k is None:
         if out_k is not None:
@@ -126,8 +128,8 @@ def _rotate(plan, q, k, positions, pairs, inverse, first, out, out_k, stream):
             _refuse(f"{who}: k is a {dtype} tensor [{B}, {L}, heads, {P}]")
         if out_k is None:
             out_k = torch.empty_like(k, memory_format=torch.contiguous_format)
-        elif out_k.dtype != dtype or out_k.shape != k_shape:
-            _refuse(f"{who}: the result of k is a {dtype} tensor {tuple(k_shape)}")
+        elif out_k.dtype != dtype or out_k.shape != k_shape or out_k.is_neg():
+            _refuse(f"{who}: the result of k is a {dtype} tensor {tuple(k_shape)}, no negated view")
         second_view = _view(who, k, out_k, k_shape[2], P)
     rc = _lib.load().tfft_rotary(
         _lib.ROTARY_ARGS.pack(_lib.ROTARY_ARGS.size, code, _PAIRS[pairs], bool(inverse), B, L, P, plan.size, plan.magnitude,
