@@ -108,12 +108,19 @@ def workspace_bytes(dtype, N, batch=1):
     return lo.value, best.value
 
 
+def lazy(t):
+    """True for a view that torch has only noted as conjugated or negated: what lies at its address are other values."""
+    return t.is_neg() or t.is_conj()
+
+
 def _points(t, N):
     """Number of complex points a tensor holds, and its TFFT dtype code."""
     if not t.is_cuda:
         raise ThunderFFTError(3, "ThunderFFT_global needs device tensors")
     if not t.is_contiguous():
         raise ThunderFFTError(3, "ThunderFFT_global needs contiguous [batch][N] interleaved data")
+    if lazy(t):
+        raise ThunderFFTError(3, "ThunderFFT_global needs the values in memory: resolve_conj() / resolve_neg() first")
     code = _DTYPE_CODE.get(t.dtype)
     if code is None:
         raise ThunderFFTError(1, f"unsupported element type {t.dtype}")

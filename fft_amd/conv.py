@@ -8,7 +8,7 @@ The same two steps are `filter_spectra` and `fft_conv` here; tensors stand in fo
 import torch
 
 from . import _lib
-from .api import ThunderFFTError, ThunderFFTInitialize, ThunderFFT_global, _check, dtype_code, exec_options
+from .api import ThunderFFTError, ThunderFFTInitialize, ThunderFFT_global, _check, dtype_code, exec_options, lazy
 
 CONV_COMPLEX, CONV_REAL_IN, CONV_REAL_IN_OUT = 0, 1, 2
 SUPPORTED_CONV_N = (4096,)
@@ -18,11 +18,18 @@ def _stream(t, stream):
     return (stream or torch.cuda.current_stream(t.device)).cuda_stream
 
 
+def _in_memory(*tensors):
+    for t in tensors:
+        if t is not None and lazy(t):
+            raise ThunderFFTError(3, "the convolutions need the values in memory: resolve_neg() first")
+
+
 def filter_layout(h_freq, N, stream=None, options=None):
     """[D, N, 2] natural-order filter spectra -> the register order the fused kernel reads (the kernel that
     `options` selects: pass the same options to fft_conv)."""
     if not (h_freq.is_cuda and h_freq.is_contiguous()) or h_freq.shape[-2:] != (N, 2):
         raise ThunderFFTError(3, "filter_layout needs a contiguous device tensor [D, N, 2]")
+    _in_memory(h_freq)
     D = h_freq.numel() // (2 * N)
     out = torch.empty_like(h_freq)
     with torch.cuda.device(h_freq.device):
@@ -61,6 +68,7 @@ def filter_spectra_fused(padded, N, stream=None):
     ThunderFFT_global followed by filter_layout. fp16, N = 4096 (ThunderFFTError UNSUPPORTED otherwise)."""
     if not (padded.is_cuda and padded.is_contiguous()) or padded.shape[-2:] != (N, 2):
         raise ThunderFFTError(3, "filter_spectra_fused needs a contiguous device tensor [D, N, 2]")
+    _in_memory(padded)
     D = padded.numel() // (2 * N)
     out = torch.empty_like(padded)
     with torch.cuda.device(padded.device):
@@ -82,6 +90,7 @@ def fft_conv(x, h_perm, N, kind=CONV_COMPLEX, out=None, stream=None, options=Non
     B, D = x.shape[0], x.shape[1]
     if h_perm.shape[0] != D or h_perm.dtype != x.dtype or not h_perm.is_contiguous():
         raise ThunderFFTError(3, "filter spectra must be contiguous [D, N, 2] of the signal's element type")
+    _in_memory(x, h_perm, out)
     if out is None:
         shape = (B, D, N) if kind == CONV_REAL_IN_OUT else (B, D, N, 2)
         out = torch.empty(shape, dtype=x.dtype, device=x.device)
@@ -121,6 +130,7 @@ def conv1d_tiled(x, hf, filter_len, N=64, out=None, stream=None):
         raise ThunderFFTError(3, f"need 1 <= filter_len <= {N} <= input length")
     if hf.dtype != x.dtype or hf.numel() != 2 * N or not hf.is_contiguous():
         raise ThunderFFTError(3, "filter spectrum must be contiguous [N, 2] of the signal's element type")
+    _in_memory(x, hf, out)
     out_len = L - filter_len + 1
     if out is None:
         out = torch.empty(out_len, 2, dtype=x.dtype, device=x.device)

@@ -214,7 +214,9 @@ class DistributedFFT:
         ops, P = self.ops, self.world
         if x_local.numel() != 2 * self.points:
             raise ValueError(f"shard holds {x_local.numel() // 2} points, expected {self.points}")
-        x = x_local.reshape(self.points, 2)
+        if out is not None and out.is_neg():
+            raise ValueError("out is a view that torch has only noted as negated")
+        x = x_local.resolve_neg().reshape(self.points, 2)
         a, b = self.buf
         self.passes = 0
 
