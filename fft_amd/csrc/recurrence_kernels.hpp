@@ -36,6 +36,7 @@ struct Chunking {
   int row = 1;           // groups whose (A, B) are joined directly; the state behind each row of groups is handed on
   int lanes = 64;        // rows: lanes that a tile fills; signals: threads of a row, where a wave holds several rows
   int each = 1;          // signals: rows of a gate that a workgroup takes one after the other
+  int side_by_side = 1;  // tiles that a workgroup holds at once; more than one only where a tile is one chunk
   bool walks = false;    // a workgroup takes all chunks of its tile, one after the other
   long long state_words = 0;  // states of one chunk
   // 64-bit words: the counters, a map a state and chunk where groups are used and a group where rows of them are, half a word a
@@ -51,7 +52,7 @@ struct Chunking {
   long long width() const { return strip && counters() > 1 ? strip : (tiles + counters() - 1) / counters(); }
   // workgroups: as many for every counter as the first one has tickets; a few find none left
   long long blocks() const {
-    if (apart() <= 1 || tiles == 0) return tiles;
+    if (apart() <= 1 || tiles == 0) return (tiles + side_by_side - 1) / side_by_side;
     const long long round = counters() * width(), rest = tiles % round;
     return counters() * (tiles / round * width() + (rest < width() ? rest : width())) * chunks;
   }

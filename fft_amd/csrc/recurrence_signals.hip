@@ -441,6 +441,7 @@ Chunking plan(long long batch, long long length, long long channels, int dtype, 
     while (c.lanes < pieces) c.lanes *= 2;
     c.waves = 4;
     c.chunks = 1;
+    c.side_by_side = 64 * c.waves / c.lanes;
   } else {
     c.walks = pieces > 64 * most && rows >= many;
     const int waves = c.walks && rows >= kShortChunks ? kWalkWaves : most;
@@ -463,11 +464,6 @@ Shape shape_of(const P& p, const Chunking& c, word* words) {
                (int)c.chunks, c.group, c.lanes, c.each, turns_of(c), words};
 }
 
-dim3 grid_of(const Chunking& c) {
-  const long long per_block = 64 * c.waves / c.lanes;
-  return dim3((unsigned)(c.lanes < 64 ? (c.tiles + per_block - 1) / per_block : c.blocks()));
-}
-
 }  // namespace
 
 bool signals_fit(const tfft_scan_args& p) {
@@ -483,12 +479,13 @@ Chunking plan_signals(const tfft_scan_grad_args& p) {
 
 void launch_signals(const tfft_scan_args& p, const Chunking& c, word* words, hipStream_t s) {
   const Shape f = shape_of(p, c, words);
+  const dim3 grid((unsigned)c.blocks()), block(64 * c.waves);
   with_types(p.dtype, p.gate_dtype, [&](auto t, auto g) {
     using T = decltype(t);
     using G = decltype(g);
-    if (c.chunks <= 1) scan_signals_fwd<T, G, ONE><<<grid_of(c), dim3(64 * c.waves), 0, s>>>(p, f);
-    else if (c.walks) scan_signals_fwd<T, G, WALK><<<grid_of(c), dim3(64 * c.waves), 0, s>>>(p, f);
-    else scan_signals_fwd<T, G, SPLIT><<<grid_of(c), dim3(64 * c.waves), 0, s>>>(p, f);
+    if (c.chunks <= 1) scan_signals_fwd<T, G, ONE><<<grid, block, 0, s>>>(p, f);
+    else if (c.walks) scan_signals_fwd<T, G, WALK><<<grid, block, 0, s>>>(p, f);
+    else scan_signals_fwd<T, G, SPLIT><<<grid, block, 0, s>>>(p, f);
   });
 }
 // Rows of parts a gate; one: none
@@ -500,11 +497,11 @@ unsigned long long signals_parts(const tfft_scan_grad_args& p) {
 void launch_signals(const tfft_scan_grad_args& p, const Chunking& c, word* words, float* parts, hipStream_t s) {
   const Shape f = shape_of(p, c, words);
   const long long pitch = pitch_of(p.length), count = parts_of_gate(p);
+  const dim3 grid((unsigned)c.blocks()), block(64 * c.waves);
   if (count == 1) parts = nullptr;
   with_types(p.dtype, p.gate_dtype, [&](auto t, auto g) {
     using T = decltype(t);
     using G = decltype(g);
-    const dim3 grid = grid_of(c), block(64 * c.waves);
     const bool shared = p.share > 1 && p.length > 0;
     if (c.chunks <= 1 && shared) scan_signals_bwd_heads<T, G><<<grid, block, 0, s>>>(p, f, parts, pitch);
     else if (c.chunks <= 1) scan_signals_bwd<T, G, ONE, false><<<grid, block, 0, s>>>(p, f, parts, pitch);
