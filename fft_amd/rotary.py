@@ -1,14 +1,15 @@
 """Rotary positions: pairs of a head's values times exp(i position frequency), and the inverse, which is the gradient.
 
-The framework's twiddle product (tfft_fourstep_twiddle) for positions and frequencies of a model's: the phase is an
-exact fraction of a turn in 64-bit integers, so positions of any size lose nothing. See tfft_rotary in
-include/thunderfft_c.h. No counterpart in the reference, whose twiddles belong to one transform
+The framework's twiddle product (tfft_fourstep_twiddle) for positions and frequencies of a model's. A frequency is rounded
+once, to a 64-bit fraction of a turn per position; the product with a 64-bit position is exact modulo one turn, so position p is
+off by p 2^-65 turns at most (2^-25 at 2^40). See tfft_rotary in include/thunderfft_c.h. No counterpart in the reference, whose twiddles belong to one transform
 (thunderfft/include/thunderfft/detail/util_arith.h:75-91).
 
     plan = RotaryPlan(128, base=10000.0)
     q, k = rotate(plan, q, k, positions)                  # q [B, L, H, P], k [B, L, H', P], positions int [B, L] or [L]
     dq, dk = rotate(plan, dq, dk, positions, inverse=True)
 """
+import functools
 import math
 
 import torch
@@ -19,6 +20,31 @@ from .recurrence import _FLOATS, _placed, _refuse, _same_device, _values
 
 _PAIRS = {"half": 0, "interleaved": 1}
 _POSITIONS = {torch.int64: 8, torch.int32: 4}
+
+
+@functools.lru_cache(maxsize=None)
+def _pi(bits):
+    """pi 2^bits to within a unit: Machin's pi = 16 atan(1/5) - 4 atan(1/239) in integers, with 32 bits more."""
+    def atan(n):
+        term = total = (1 << bits + 32) // n
+        k = 1
+        while term:
+            term //= -n * n
+            k += 2
+            total += term // k
+        return total
+
+    return 16 * atan(5) - 4 * atan(239) >> 32
+
+
+def _word(f):
+    """round(2^64 f / (2 pi)) modulo 2^64 for any fp64 number f, as a signed 64-bit number. The quotient is right to 2^-64 with
+    64 bits of pi more than it has itself."""
+    bits = 192 if abs(f) < 2.0 ** 64 else 1152
+    n, d = f.as_integer_ratio()
+    over, under = n << 64 + bits, d * _pi(bits) * 2
+    word = (2 * over + under) // (2 * under) % 2 ** 64
+    return word - 2 ** 64 if word >= 2 ** 63 else word
 
 
 class RotaryPlan:
@@ -65,10 +91,8 @@ class RotaryPlan:
         if not math.isfinite(magnitude):
             _refuse("RotaryPlan: magnitude is finite")
         self.size, self.magnitude, self.frequencies = size, float(magnitude), frequencies
-        # turns per position in units of 2^-64, modulo 1 turn; the fp64 quotient is exact to 2^-53 of itself
-        words = [int(f / (2.0 * math.pi) % 1.0 * 2.0 ** 64) % 2 ** 64 for f in frequencies]
-        words = [w - 2 ** 64 if w >= 2 ** 63 else w for w in words]
-        self.turns = torch.tensor(words, dtype=torch.int64).to("cuda" if device is None else device)
+        # turns per position in units of 2^-64, modulo 1 turn
+        self.turns = torch.tensor([_word(f) for f in frequencies], dtype=torch.int64).to("cuda" if device is None else device)
 
 
 def rotate(plan, q, k=None, positions=None, pairs="half", inverse=False, first=0, out=None, out_k=None, stream=None):

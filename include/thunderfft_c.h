@@ -379,8 +379,9 @@ int tfft_scan_step(const tfft_scan_step_args* args, void* stream);
 /* Rotary positions: the pair (re, im) number i of every head of the token at position p becomes
  *     magnitude * (re + i im) * exp(2 pi i p F[i]),    conjugated when inverse != 0 (which makes it the gradient),
  * the product of tfft_fourstep_twiddle with frequencies and positions of the caller's. turns: rotary / 2 device words
- * of 64 bits, the frequency in units of 2^-64 turns per position, round(2^64 f / 2 pi) for f radians per position: the
- * product with a 64-bit position, taken modulo 2^64, is the phase to 2^-64 turns times the position, however far it is.
+ * of 64 bits, the frequency in units of 2^-64 turns per position, round(2^64 f / 2 pi) modulo 2^64 for f radians per
+ * position: the product with a 64-bit position, taken modulo 2^64, is that frequency's phase exactly, and f's to 2^-65 turns
+ * times the position.
  * pairs TFFT_PAIRS_HALF: values i and i + rotary / 2 of the head; TFFT_PAIRS_INTERLEAVED: values 2 i and 2 i + 1.
  * Values behind the first `rotary` of a head are copied. Rotates one tensor or two (the second one's in NULL) by the
  * same positions in one launch; element strides (batch, time, head), values of a head contiguous; out may be in with
