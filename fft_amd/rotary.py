@@ -69,9 +69,14 @@ class RotaryPlan:
                 _refuse("RotaryPlan: base and factor are positive")
             if scaling not in (None, "linear", "base", "ramp"):
                 _refuse(f"RotaryPlan: unknown scaling {scaling!r} (None, 'linear', 'base' or 'ramp')")
-            if scaling == "base" and size > 2:
-                base = base * factor ** (size / (size - 2.0))
-            frequencies = [base ** (-2.0 * i / size) for i in range(size // 2)]
+            try:
+                if scaling == "base" and size > 2:
+                    base = base * factor ** (size / (size - 2.0))
+                frequencies = [base ** (-2.0 * i / size) for i in range(size // 2)]
+            except (OverflowError, ZeroDivisionError):
+                base = math.inf
+            if not math.isfinite(base):
+                _refuse("RotaryPlan: base and factor leave the range of fp64")
             if scaling == "linear":
                 frequencies = [f / factor for f in frequencies]
             if scaling == "ramp":
@@ -88,8 +93,8 @@ class RotaryPlan:
         frequencies = [float(f) for f in frequencies]
         if len(frequencies) != size // 2 or not all(math.isfinite(f) for f in frequencies):
             _refuse(f"RotaryPlan: {size // 2} finite frequencies")
-        if not math.isfinite(magnitude):
-            _refuse("RotaryPlan: magnitude is finite")
+        if not abs(magnitude) <= torch.finfo(torch.float32).max:
+            _refuse("RotaryPlan: magnitude is a finite fp32 number")
         self.size, self.magnitude, self.frequencies = size, float(magnitude), frequencies
         # turns per position in units of 2^-64, modulo 1 turn
         self.turns = torch.tensor([_word(f) for f in frequencies], dtype=torch.int64).to("cuda" if device is None else device)
@@ -126,7 +131,12 @@ def _rotate(plan, q, k, positions, pairs, inverse, first, out, out_k, stream):
     if plan.size > P:
         _refuse(f"{who}: the plan rotates {plan.size} values, a head has {P}")
     at = position_bytes = position_batch = position_time = 0
-    if positions is not None:
+    if positions is None:
+        first = int(first)
+        if not -2 ** 63 <= first < 2 ** 63:
+            _refuse(f"{who}: first is a 64-bit number, not {first}")
+    else:
+        first = 0
         position_bytes = _POSITIONS.get(positions.dtype)
         if position_bytes is None:
             _refuse(f"{who}: positions are int64 or int32, not {positions.dtype}")
@@ -157,7 +167,7 @@ def _rotate(plan, q, k, positions, pairs, inverse, first, out, out_k, stream):
         second_view = _view(who, k, out_k, k_shape[2], P)
     rc = _lib.load().tfft_rotary(
         _lib.ROTARY_ARGS.pack(_lib.ROTARY_ARGS.size, code, _PAIRS[pairs], bool(inverse), B, L, P, plan.size, plan.magnitude,
-                              position_bytes, plan.turns.data_ptr(), at, position_batch, position_time, int(first),
+                              position_bytes, plan.turns.data_ptr(), at, position_batch, position_time, first,
                               *first_view, *second_view), stream)
     if rc:
         _check(rc)
