@@ -13,6 +13,7 @@ tfft_scan_backward and tfft_scan_step (include/thunderfft_c.h).
 import ctypes
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .api import ThunderFFTError, _check
@@ -50,9 +51,9 @@ def _types(who, x, gate):
 
 def _same_device(who, x, *others):
     """Index of the device that all tensors lie on"""
-    if not x.is_cuda:
-        _refuse(f"{who} needs device tensors")
     device = x.get_device()
+    if device < 0:
+        _refuse(f"{who} needs device tensors")
     for t in others:
         if t is not None and t.get_device() != device:
             _refuse(f"{who}: tensors on {x.device} and {t.device}")
@@ -104,6 +105,7 @@ def _out(who, name, t, like):
         return torch.empty_like(like, memory_format=torch.contiguous_format)
     if t.dtype != like.dtype or t.shape != like.shape or t.is_neg():
         _refuse(f"{who}: {name} is a {like.dtype} tensor {tuple(like.shape)}, no negated view")
+    increment_version(t)  # a tensor that autograd has saved and that is written into counts as changed
     return t
 
 
@@ -191,11 +193,11 @@ def gated_scan_step(x, gate, state, log_gate=False, new_state=None, out=None, st
 def _gated_scan_step(x, gate, state, log_gate, new_state, out, stream):
     who = "gated_scan_step"
     code, gate_code = _types(who, x, gate)
-    if x.dim() != 2 or gate.dim() != 2 or gate.shape[0] != x.shape[0]:
-        _refuse(f"{who} needs x [B, D] and gate [B, G], got {tuple(x.shape)} and {tuple(gate.shape)}")
-    shape = x.shape
+    shape, gates = x.shape, gate.shape
+    if len(shape) != 2 or len(gates) != 2 or gates[0] != shape[0]:
+        _refuse(f"{who} needs x [B, D] and gate [B, G], got {tuple(shape)} and {tuple(gates)}")
     B, D = shape
-    G = gate.shape[1]
+    G = gates[1]
     if D > 0 if G < 1 else D % G:
         _refuse(f"{who}: {G} gates do not divide {D} channels")
     if new_state is None:
@@ -219,4 +221,5 @@ def _gated_scan_step(x, gate, state, log_gate, new_state, out, stream):
                                  gate.data_ptr(), state.data_ptr(), new_state.data_ptr(), y.data_ptr(), *rows), stream)
     if rc:
         _check(rc)
+    increment_version(new_state)
     return y

@@ -16,7 +16,7 @@ import torch
 
 from . import _lib
 from .api import _check
-from .recurrence import _FLOATS, _placed, _refuse, _same_device, _values
+from .recurrence import _FLOATS, _out, _placed, _refuse, _same_device, _values
 
 _PAIRS = {"half": 0, "interleaved": 1}
 _POSITIONS = {torch.int64: 8, torch.int32: 4}
@@ -147,10 +147,7 @@ def _rotate(plan, q, k, positions, pairs, inverse, first, out, out_k, stream):
         else:
             _refuse(f"{who}: positions {tuple(positions.shape)} are neither [{B}, {L}] nor [{L}]")
         at = positions.data_ptr()
-    if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif out.dtype != dtype or out.shape != shape or out.is_neg():
-        _refuse(f"{who}: the result of q is a {dtype} tensor {tuple(shape)}, no negated view")
+    out = _out(who, "the result of q", out, q)
     first_view = _view(who, q, out, H, P)
     if k is None:
         if out_k is not None:
@@ -160,10 +157,7 @@ def _rotate(plan, q, k, positions, pairs, inverse, first, out, out_k, stream):
         k_shape = k.shape
         if k.dtype != dtype or len(k_shape) != 4 or k_shape[0] != B or k_shape[1] != L or k_shape[3] != P:
             _refuse(f"{who}: k is a {dtype} tensor [{B}, {L}, heads, {P}]")
-        if out_k is None:
-            out_k = torch.empty_like(k, memory_format=torch.contiguous_format)
-        elif out_k.dtype != dtype or out_k.shape != k_shape or out_k.is_neg():
-            _refuse(f"{who}: the result of k is a {dtype} tensor {tuple(k_shape)}, no negated view")
+        out_k = _out(who, "the result of k", out_k, k)
         second_view = _view(who, k, out_k, k_shape[2], P)
     rc = _lib.load().tfft_rotary(
         _lib.ROTARY_ARGS.pack(_lib.ROTARY_ARGS.size, code, _PAIRS[pairs], bool(inverse), B, L, P, plan.size, plan.magnitude,
