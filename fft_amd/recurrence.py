@@ -9,8 +9,12 @@ tfft_scan_backward and tfft_scan_step (include/thunderfft_c.h).
     y, last = gated_scan(x, gate, dim=2)                        # the convolution's signals: x [B, D, L], gate [B, G, L]
     dx, dgate, dinitial = gated_scan_backward(dy, y, gate)      # y as gated_scan returned it
     y = gated_scan_step(x, gate, state)                         # x [B, D], gate [B, G], state fp32 [B, D], in place
+
+Autograd does not see these calls: a torch.autograd.Function around gated_scan saves y and calls gated_scan_backward. Outside
+one, a tensor that requires a gradient is taken for its values, with a warning while gradients are enabled.
 """
 import ctypes
+import warnings
 
 import torch
 from torch.autograd.graph import increment_version
@@ -50,13 +54,19 @@ def _types(who, x, gate):
 
 
 def _same_device(who, x, *others):
-    """Index of the device that all tensors lie on"""
-    device = x.get_device()
+    """Index of the device that all tensors lie on. Says so where the call cuts off the graph of one of them."""
+    device, tracked = x.get_device(), x.requires_grad
     if device < 0:
         _refuse(f"{who} needs device tensors")
     for t in others:
-        if t is not None and t.get_device() != device:
-            _refuse(f"{who}: tensors on {x.device} and {t.device}")
+        if t is not None:
+            if t.get_device() != device:
+                _refuse(f"{who}: tensors on {x.device} and {t.device}")
+            if t.requires_grad:
+                tracked = True
+    if tracked and torch.is_grad_enabled():
+        warnings.warn(f"{who}: autograd does not see this call, its results are cut off from the graph of a tensor that requires a "
+                      "gradient (call it in a torch.autograd.Function, or under torch.no_grad())", stacklevel=3)
     return device
 
 
@@ -140,7 +150,7 @@ def gated_scan(x, gate, dim=1, log_gate=False, lengths=None, initial=None, out=N
 
 def _gated_scan(x, gate, dim, log_gate, lengths, initial, out, stream):
     who = "gated_scan"
-    if any(t is not None and t.is_neg() for t in (x, gate, lengths, initial)):
+    if x.is_neg() or gate.is_neg() or (lengths is not None and lengths.is_neg()) or (initial is not None and initial.is_neg()):
         x, gate, lengths, initial = _values(x, gate, lengths, initial)
     code, gate_code = _types(who, x, gate)
     B, L, D, share = _sizes(who, x, gate, dim)
@@ -167,7 +177,7 @@ def gated_scan_backward(dy, y, gate, dim=1, log_gate=False, lengths=None, initia
 
 def _gated_scan_backward(dy, y, gate, dim, log_gate, lengths, initial, dlast, dx, dgate, stream):
     who = "gated_scan_backward"
-    if any(t is not None and t.is_neg() for t in (dy, y, gate, lengths, initial, dlast)):
+    if dy.is_neg() or y.is_neg() or gate.is_neg() or any([t.is_neg() for t in (lengths, initial, dlast) if t is not None]):
         dy, y, gate, lengths, initial, dlast = _values(dy, y, gate, lengths, initial, dlast)
     code, gate_code = _types(who, dy, gate)
     B, L, D, share = _sizes(who, dy, gate, dim)

@@ -8,6 +8,9 @@ off by p 2^-65 turns at most (2^-25 at 2^40). See tfft_rotary in include/thunder
     plan = RotaryPlan(128, base=10000.0)
     q, k = rotate(plan, q, k, positions)                  # q [B, L, H, P], k [B, L, H', P], positions int [B, L] or [L]
     dq, dk = rotate(plan, dq, dk, positions, inverse=True)
+
+Autograd does not see these calls; a tensor that requires a gradient is taken for its values, with a warning while gradients are
+enabled (the gradient is the inverse rotation, in a torch.autograd.Function).
 """
 import functools
 import math
