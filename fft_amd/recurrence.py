@@ -140,7 +140,8 @@ def gated_scan(x, gate, dim=1, log_gate=False, lengths=None, initial=None, out=N
     """(y, last): the recurrence over dimension `dim` of x, and the fp32 state [B, D] behind the last step.
 
     x: [B, L, D] (dim = 1) or [B, D, L] (dim = 2), float32, float16 or bfloat16, any strides. gate: the same with G
-    channels, one for D / G neighbours, of x's type or float32; with log_gate the decay is exp(gate). lengths (int32
+    channels, one for D / G neighbours, of x's type or float32; with log_gate the decay is exp(gate). Decays above 1 need
+    a product over every stretch of steps, restarts or not, that is finite in fp32 (tfft_scan_forward). lengths (int32
     [B]): steps behind a sequence's length do not count, leave the state as it is, and y is 0 there. initial: fp32
     [B, D]. out: a tensor for y, x itself allowed. Inputs count by their values, a negation that torch has only noted
     (z.conj().imag) included; into such a view nothing is written. Asynchronous on `stream` (default: torch's current stream)."""

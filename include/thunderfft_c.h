@@ -304,8 +304,10 @@ int tfft_get_twiddle_table(int dtype, int n, const void** d_table);
  * rounded once. gate_form TFFT_GATE_DECAY: a = gate; TFFT_GATE_LOG: a = exp(gate), a gate of minus infinity restarts
  * the recurrence, whatever finite state it has (like a decay of 0; 0 times infinity is NaN). `share` consecutive
  * channels share one gate: the gate has channels / share entries a step (share divides channels). |a| <= 1 is what the
- * operator is made for; larger decays are computed as long as the product of the decays over the sequence stays finite
- * in fp32.
+ * operator is made for. Larger decays are computed as long as for every stretch of consecutive steps, wherever it begins and
+ * ends, the product of its decays and the states that it reaches from zero stay finite in fp32: stretches are computed apart
+ * and joined, so a product that overflows gives infinity or NaN also behind a state that is small enough to bear it, and a
+ * restart (a decay of 0) in front of it does not lift this. Only states of exactly zero are kept out of such products.
  *
  * Layout: element strides (batch, time, channel; for the gate: batch, time, gate). Any non-negative strides are taken;
  * inputs may repeat (stride 0), outputs may not. Layouts with kernels of their own are channel stride 1 ([batch][time]
