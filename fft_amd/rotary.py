@@ -26,8 +26,8 @@ _POSITIONS = {torch.int64: 8, torch.int32: 4}
 
 
 @functools.lru_cache(maxsize=None)
-def _pi(bits):
-    """pi 2^bits to within a unit: Machin's pi = 16 atan(1/5) - 4 atan(1/239) in integers, with 32 bits more."""
+def _one_turn(bits):
+    """2^bits / (2 pi) to within a few units, with pi by Machin's formula 16 atan(1/5) - 4 atan(1/239) in integers and 32 bits more"""
     def atan(n):
         term = total = (1 << bits + 32) // n
         k = 1
@@ -37,16 +37,16 @@ def _pi(bits):
             total += term // k
         return total
 
-    return 16 * atan(5) - 4 * atan(239) >> 32
+    return (1 << 2 * bits + 31) // (16 * atan(5) - 4 * atan(239))
 
 
 def _word(f):
-    """round(2^64 f / (2 pi)) modulo 2^64 for any fp64 number f, as a signed 64-bit number. The quotient is right to 2^-64 with
-    64 bits of pi more than it has itself."""
-    bits = 192 if abs(f) < 2.0 ** 64 else 1152
-    n, d = f.as_integer_ratio()
-    over, under = n << 64 + bits, d * _pi(bits) * 2
-    word = (2 * over + under) // (2 * under) % 2 ** 64
+    """round(2^64 f / (2 pi)) modulo 2^64 for any fp64 number f, as a signed 64-bit number. f is m 2^e with 53 bits of m; the
+    product with so many bits of 1 / (2 pi) is right to 2^-120 before it is rounded."""
+    m, e = math.frexp(f)
+    bits = 256 if e <= 64 else 1216
+    shift = bits - 11 - e  # at least 181
+    word = (int(m * 2.0 ** 53) * _one_turn(bits) + (1 << shift - 1) >> shift) % 2 ** 64
     return word - 2 ** 64 if word >= 2 ** 63 else word
 
 
