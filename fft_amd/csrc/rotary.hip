@@ -30,7 +30,7 @@ __device__ __forceinline__ void turn(uint64_t phase, float* c, float* s) {
   }
 }
 
-// What bounds it: HBM. 8 x 4096 tokens with 32 + 8 heads of 128 in bf16 take 118 us (671 MB, 5.7 TB/s); the factors, evaluated in
+// What bounds it: HBM. 8 x 4096 tokens with 32 + 8 heads of 128 in bf16 take 116 us (671 MB, 5.8 TB/s); the factors, evaluated in
 // registers from 8 bytes a pair, hide behind it. One token each of 64 sequences takes 4 us, a launch and its latency.
 //
 // A unit is what a thread holds of one head: R values of each half (pairs i, i + rotary / 2), twice as many pairs, or R values
@@ -144,8 +144,9 @@ __global__ __launch_bounds__(256) void rotary_units(tfft_rotary_args p, Grid g) 
   }
 }
 
-// Heads whose factors a thread shares: 8 x 4096 tokens with 32 + 8 heads of 128 in bf16 take 158, 130, 125, 126, 129 us with
-// 1, 2, 4, 5, 8. Calls that would be left with fewer than kEnough threads (256 CUs of 1024) give every head its own.
+// Heads whose factors a thread shares: 8 x 4096 tokens with 32 + 8 heads of 128 in bf16 take 153, 119, 116, 121, 123 us with
+// 1, 2, 4, 5, 8, 5 x 2489 with 21 heads of 174 in fp16 58, 51, 49, 49, 50. Calls that would be left with fewer than kEnough
+// threads (256 CUs of 1024) give every head its own.
 constexpr int kHeads = 4;
 constexpr long long kEnough = 256 * 1024, kMost = 1LL << 30;
 
@@ -169,8 +170,8 @@ extern "C" int tfft_rotary(const tfft_rotary_args* args, void* stream) {
   if (!p.tensor[1].in) p.tensor[1].heads = 0;
   if (p.batch > kMost || p.length > kMost || p.head > kMost || p.tensor[0].heads > kMost / 4 || p.tensor[1].heads > kMost / 4)
     return refuse("an extent is too large");
-  // Results that leave in whole lines and whole units are streamed: 8 x 4096 tokens with 32 + 8 heads of 128 in bf16 119 us
-  // against 126, 9003 tokens with 12 heads of 96 in fp32 15 against 17.
+  // Results that leave in whole lines and whole units are streamed: 8 x 4096 tokens with 32 + 8 heads of 128 in bf16 116 us
+  // against 126, 160000 tokens with 12 heads of 96 in fp32 269 against 288.
   const long long size = p.dtype == TFFT_F32 ? 4 : 2;
   bool in_place = true, stream_out = p.rotary / 2 * size % 16 == 0 && p.head * size % 16 == 0;
   for (const tfft_rotary_view& v : p.tensor) {
