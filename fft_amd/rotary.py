@@ -2,8 +2,8 @@
 
 The framework's twiddle product (tfft_fourstep_twiddle) for positions and frequencies of a model's. A frequency is rounded
 once, to a 64-bit fraction of a turn per position; the product with a 64-bit position is exact modulo one turn, so position p is
-off by p 2^-65 turns at most (2^-25 at 2^40). See tfft_rotary in include/thunderfft_c.h. No counterpart in the reference, whose twiddles belong to one transform
-(thunderfft/include/thunderfft/detail/util_arith.h:75-91).
+off by p 2^-65 turns at most (2^-25 at 2^40). See tfft_rotary in include/thunderfft_c.h. No counterpart in the reference, whose
+twiddles belong to one transform (thunderfft/include/thunderfft/detail/util_arith.h:75-91).
 
     plan = RotaryPlan(128, base=10000.0)
     q, k = rotate(plan, q, k, positions)                  # q [B, L, H, P], k [B, L, H', P], positions int [B, L] or [L]
@@ -109,8 +109,9 @@ def rotate(plan, q, k=None, positions=None, pairs="half", inverse=False, first=0
     q, k: [B, L, heads, P] float32, float16 or bfloat16 with contiguous heads, heads of their own number; the first
     plan.size of the P values are rotated, the rest copied. pairs: "half" pairs value i with i + size / 2, "interleaved"
     2 i with 2 i + 1. positions: int64 or int32 [B, L] or [L] on the device (negative ones turn backwards); without
-    them position t is first + t. inverse: the other way round, which is the gradient of rotate. out, out_k: tensors for the results,
-    q and k themselves allowed (but no view that torch has only noted as negated). Asynchronous on `stream` (default: torch's current stream)."""
+    them position t is first + t. inverse: the other way round, which is the gradient of rotate. out, out_k: tensors for the
+    results, q and k themselves allowed (but no view that torch has only noted as negated). Asynchronous on `stream` (default:
+    torch's current stream)."""
     device = _same_device("rotate", q, k, plan.turns, positions, out, out_k)
     return _placed(_rotate, device, stream, plan, q, k, positions, pairs, inverse, first, out, out_k)
 
